@@ -1,6 +1,7 @@
 /*
  * sessd3d.h -- C-ABI of the MI355X (gfx950) implementation of the SE-SSD 3-D front end:
- * voxelGenerator, SubmConv3dLayer, SparseConv3dLayer and sparse2Dense.
+ * voxelGenerator, SubmConv3dLayer, SparseConv3dLayer and sparse2Dense; beside them the layers of a transformer block over
+ * the same voxel features (RmsNorm, Linear8, VoxelAttention), which the reference does not have.
  *
  * One set of entry points per layer type.  Each set mirrors the life cycle TensorRT drives on
  * the reference's IPluginV2DynamicExt plugins:
@@ -42,8 +43,9 @@ typedef void* sessd_stream_t; /* a hipStream_t; NULL = the default stream */
  * sits behind that queue's kernels. */
 #define SESSD_STREAM_NONE ((sessd_stream_t)(intptr_t)-1)
 
-/* Values follow nvinfer1::DataType so descriptors can be copied field by field. */
-enum { SESSD_FLOAT = 0, SESSD_HALF = 1, SESSD_INT32 = 3 };
+/* Values follow nvinfer1::DataType so descriptors can be copied field by field.  SESSD_FP8 is e4m3 without infinities
+ * (largest value 448), as the rows of RmsNormPlugin and Linear8Plugin are held in. */
+enum { SESSD_FLOAT = 0, SESSD_HALF = 1, SESSD_INT32 = 3, SESSD_FP8 = 6 };
 
 /* Mirrors nvinfer1::PluginTensorDesc {Dims dims; DataType type; TensorFormat format; float scale;}
  * (format is always 0 = kLINEAR here). */
@@ -324,6 +326,118 @@ int sessd_sparse2dense_set_padding(sessd_sparse2dense* h, int32_t top, int32_t b
 void sessd_sparse2dense_destroy(sessd_sparse2dense* h);
 
 /* ------------------------------------------------------------------------------------------ */
+/* RmsNormPlugin, Linear8Plugin, VoxelAttentionPlugin   (no counterpart in the reference)      */
+/* ------------------------------------------------------------------------------------------ */
+/* The layers of a transformer block over voxel features: a norm that takes the residual in and leaves its rows in 8
+ * bits, the projection that reads such rows, and attention among the voxels of a window.  Life cycle, tensors, streams
+ * and errors are those of the layers above; the first two need no workspace (workspace_size is 0, NULL is accepted).
+ * Rows beyond voxel_num: zeros, or what Linear8's epilogue makes of zeros; left as they were with
+ * SESSD_FLAG_SKIP_PAD_ROWS. */
+
+/* inputs : 0 feat [1,max_voxels,C] f32|f16   1 voxel_num i32[1]   [2 residual, as feat]
+ * outputs: 0 q fp8 [1,max_voxels,C]   1 scale f32 [1,max_voxels,1]   [2 sum, as feat]
+ * h = feat + residual, y = gamma * h / sqrt(mean over C of h^2 + eps), scale = max(max|y| / 448, 2^-100),
+ * q = y / scale to the nearest e4m3, sum = h.  All of it is computed in FP32 from the unrounded h.  A row with a value
+ * that is not finite, or whose mean of h^2 is not (|h| from about 1e19), leaves nothing that counts: its scale is NaN and
+ * all of its q are.  `sum` may be the tensor `feat` or `residual`; no other output may overlap an input.
+ * With two inputs there are two outputs, with three three.  channel: 1 .. 4096, multiples of 8 are fastest. */
+typedef struct sessd_rmsnorm sessd_rmsnorm;
+
+typedef struct sessd_rmsnorm_desc {
+    int32_t channel;
+    int32_t max_voxels;
+    float eps; /* >= 0 */
+} sessd_rmsnorm_desc;
+
+/* gamma: host FP32 [channel], finite */
+int sessd_rmsnorm_create(const sessd_rmsnorm_desc* desc, const float* gamma, sessd_rmsnorm** out);
+int sessd_rmsnorm_deserialize(const void* bytes, size_t n, sessd_rmsnorm** out);
+size_t sessd_rmsnorm_serialization_size(const sessd_rmsnorm* h);
+int sessd_rmsnorm_serialize(const sessd_rmsnorm* h, void* buf);
+int sessd_rmsnorm_configure(sessd_rmsnorm* h, const sessd_tensor_desc* in, int nIn, const sessd_tensor_desc* out, int nOut);
+size_t sessd_rmsnorm_workspace_size(const sessd_rmsnorm* h, const sessd_tensor_desc* in, int nIn,
+                                    const sessd_tensor_desc* out, int nOut);
+int sessd_rmsnorm_enqueue(sessd_rmsnorm* h, const sessd_tensor_desc* inDesc, const sessd_tensor_desc* outDesc,
+                          const void* const* inputs, void* const* outputs, void* workspace, sessd_stream_t stream);
+int sessd_rmsnorm_set_flags(sessd_rmsnorm* h, int32_t flags);
+void sessd_rmsnorm_destroy(sessd_rmsnorm* h);
+
+/* inputs : 0 q fp8 [1,max_voxels,Cin]   1 scale f32 [1,max_voxels,1]   2 voxel_num i32[1]
+ * outputs: 0 feat [1,max_voxels,Cout] f32|f16
+ * feat = (q . Wq) * scale * wscale, then the epilogue of the convolutions (x * scale[c] + shift[c], ReLU; NaN stays).
+ * The weights are rounded once, at create: wscale[c] = max(max|W[.][c]| / 448, 2^-100), Wq = W / wscale to
+ * the nearest e4m3.  Products are exact, sums FP32.  Cin: multiples of 16 up to 4096, Cout: 1 .. 4096. */
+typedef struct sessd_linear8 sessd_linear8;
+
+typedef struct sessd_linear8_desc {
+    int32_t in_channel;
+    int32_t out_channel;
+    int32_t max_voxels;
+} sessd_linear8_desc;
+
+/* weights: host FP32 [Cin][Cout], finite */
+int sessd_linear8_create(const sessd_linear8_desc* desc, const float* weights, sessd_linear8** out);
+int sessd_linear8_deserialize(const void* bytes, size_t n, sessd_linear8** out);
+size_t sessd_linear8_serialization_size(const sessd_linear8* h);
+int sessd_linear8_serialize(const sessd_linear8* h, void* buf);
+int sessd_linear8_configure(sessd_linear8* h, const sessd_tensor_desc* in, int nIn, const sessd_tensor_desc* out, int nOut);
+size_t sessd_linear8_workspace_size(const sessd_linear8* h, const sessd_tensor_desc* in, int nIn,
+                                    const sessd_tensor_desc* out, int nOut);
+int sessd_linear8_enqueue(sessd_linear8* h, const sessd_tensor_desc* inDesc, const sessd_tensor_desc* outDesc,
+                          const void* const* inputs, void* const* outputs, void* workspace, sessd_stream_t stream);
+/* As sessd_submconv3d_set_epilogue. */
+int sessd_linear8_set_epilogue(sessd_linear8* h, const float* scale, const float* shift, int relu);
+int sessd_linear8_set_flags(sessd_linear8* h, int32_t flags);
+void sessd_linear8_destroy(sessd_linear8* h);
+
+/* inputs : 0 qkv [1,max_voxels,(num_heads + 2 * num_kv_heads) * head_dim] f32|f16: queries, keys, values
+ *          1 coors i32[1,max_voxels,4]   2 voxel_num i32[1]
+ * outputs: 0 feat [1,max_voxels,num_heads * head_dim], as qkv
+ * Voxel i attends to the voxels j of its own window, itself among them: those with the same
+ * (coor + window_shift) / window_shape on every axis.  Query head h reads key and value head h * num_kv_heads / num_heads.
+ *     score = softmax_scale * q_i . k_j;   score = score_cap * tanh(score / score_cap) if score_cap > 0;
+ *     score -= slope[h] * |p_i - p_j|,  p = coor * cell_size (Euclidean distance of the voxels' centres);
+ *     feat_i = sum over j of softmax_j(score) * v_j
+ * Scores, softmax and sums are FP32; with FP16 tensors the weights are rounded to FP16 in front of their product with v.
+ * A row whose coordinates lie outside the grid takes part in nothing, its output is zeros and SESSD_STATUS_BAD_COORD is
+ * raised.  Rows that name one voxel are all of them rows of its window.  No value of another window reaches a row, whatever
+ * it is.  The order of a row's sums follows from the window's rows alone: ascending. */
+typedef struct sessd_voxelattn sessd_voxelattn;
+
+typedef struct sessd_voxelattn_desc {
+    int32_t num_heads;        /* a multiple of num_kv_heads */
+    int32_t num_kv_heads;
+    int32_t head_dim;         /* a multiple of 8, up to 128 */
+    int32_t max_voxels;
+    int32_t spatial_shape[3]; /* x,y,z */
+    int32_t window_shape[3];  /* x,y,z, cells; at most 2^22 windows in the grid */
+    int32_t window_shift[3];  /* x,y,z, 0 .. window_shape - 1 */
+    float cell_size[3];       /* x,y,z: of a cell, in the unit that the slopes are per */
+    float softmax_scale;      /* 0 = 1 / sqrt(head_dim) */
+    float score_cap;          /* 0 = none */
+} sessd_voxelattn_desc;
+
+/* slopes: host FP32 [num_heads], finite, or NULL for no bias */
+int sessd_voxelattn_create(const sessd_voxelattn_desc* desc, const float* slopes, sessd_voxelattn** out);
+int sessd_voxelattn_deserialize(const void* bytes, size_t n, sessd_voxelattn** out);
+size_t sessd_voxelattn_serialization_size(const sessd_voxelattn* h);
+int sessd_voxelattn_serialize(const sessd_voxelattn* h, void* buf);
+int sessd_voxelattn_configure(sessd_voxelattn* h, const sessd_tensor_desc* in, int nIn, const sessd_tensor_desc* out, int nOut);
+size_t sessd_voxelattn_workspace_size(const sessd_voxelattn* h, const sessd_tensor_desc* in, int nIn,
+                                      const sessd_tensor_desc* out, int nOut);
+int sessd_voxelattn_enqueue(sessd_voxelattn* h, const sessd_tensor_desc* inDesc, const sessd_tensor_desc* outDesc,
+                            const void* const* inputs, void* const* outputs, void* workspace, sessd_stream_t stream);
+/* The layer on the windows that an earlier sessd_voxelattn_enqueue left in `window_workspace` (same coors, voxel_num,
+ * max_voxels, spatial_shape, window_shape and window_shift; heads, slopes and the rest may differ): consecutive layers on
+ * one coors tensor find their windows once.  The same bits as sessd_voxelattn_enqueue. */
+int sessd_voxelattn_enqueue_shared(sessd_voxelattn* h, const sessd_tensor_desc* inDesc, const sessd_tensor_desc* outDesc,
+                                   const void* const* inputs, void* const* outputs, const void* window_workspace,
+                                   sessd_stream_t stream);
+int sessd_voxelattn_set_flags(sessd_voxelattn* h, int32_t flags);
+int sessd_voxelattn_status(const sessd_voxelattn* h, const void* workspace, sessd_stream_t stream, int32_t* status);
+void sessd_voxelattn_destroy(sessd_voxelattn* h);
+
+/* ------------------------------------------------------------------------------------------ */
 /* Creators by name and clone()  (reference: the four XxxPluginCreator classes and               */
 /* IPluginV2DynamicExt::clone, e.g. submConv3dlayer.cu:732-878, 188-196)                         */
 /* ------------------------------------------------------------------------------------------ */
@@ -348,13 +462,16 @@ typedef struct sessd_plugin_field_collection {
  * sparseConv3dlayer.cu:918-954, sparse2Dense.cu:316-341): the fields createPlugin reads, `data` NULL,
  * `length` = the number of elements it reads (0 for weights: the layer shape decides).  plugin_name is the
  * reference's PLUGIN_NAME: "VoxelGeneratorPlugin", "SubmConv3dLayerPlugin", "SparseConv3dLayerPlugin",
- * "Sparse2DensePlugin".  NULL for any other name. */
+ * "Sparse2DensePlugin".  This library's own are "RmsNormPlugin", "Linear8Plugin" and "VoxelAttentionPlugin"; their fields
+ * are named as those of their descs, with the weights last ("gamma", "weights", "slopes": num_heads values, zeros for no
+ * bias).  NULL for any other name. */
 const sessd_plugin_field_collection* sessd_plugin_field_names(const char* plugin_name);
 /* replaces XxxPluginCreator::createPlugin(name, fc) (voxelGenerator.cu:649-701, submConv3dlayer.cu:770-878,
  * sparseConv3dlayer.cu:956-1079, sparse2Dense.cu:343-373): fields are picked by name, in any order, unknown
  * names are ignored; a missing field or a field of the wrong type is an error (the reference builds the
  * plugin from zeros).  Array fields may carry length 1, as the reference's own creators declare them.
- * *handle is a sessd_voxelgen* / sessd_submconv3d* / sessd_sparseconv3d* / sessd_sparse2dense*. */
+ * *handle is a sessd_voxelgen* / sessd_submconv3d* / sessd_sparseconv3d* / sessd_sparse2dense* / sessd_rmsnorm* /
+ * sessd_linear8* / sessd_voxelattn*. */
 int sessd_plugin_create(const char* plugin_name, const sessd_plugin_field_collection* fc, void** handle);
 /* replace clone() (voxelGenerator.cu:152-159, submConv3dlayer.cu:188-196, sparseConv3dlayer.cu:204-210,
  * sparse2Dense.cu:120-125): an independent plugin with its own device copy of the weights, plus what this
@@ -363,6 +480,9 @@ int sessd_voxelgen_clone(const sessd_voxelgen* h, sessd_voxelgen** out);
 int sessd_submconv3d_clone(const sessd_submconv3d* h, sessd_submconv3d** out);
 int sessd_sparseconv3d_clone(const sessd_sparseconv3d* h, sessd_sparseconv3d** out);
 int sessd_sparse2dense_clone(const sessd_sparse2dense* h, sessd_sparse2dense** out);
+int sessd_rmsnorm_clone(const sessd_rmsnorm* h, sessd_rmsnorm** out);
+int sessd_linear8_clone(const sessd_linear8* h, sessd_linear8** out);
+int sessd_voxelattn_clone(const sessd_voxelattn* h, sessd_voxelattn** out);
 
 /* ------------------------------------------------------------------------------------------ */
 /* Frame pipeline: voxelGenerator -> SpMiddleFHD conv stack (+BN+ReLU) -> sparse2Dense          */

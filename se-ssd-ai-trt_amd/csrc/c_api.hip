@@ -12,6 +12,12 @@ using namespace sessd;
 #define H_SUBM(h) reinterpret_cast<SubmConv3dLayerPlugin*>(h)
 #define H_SP(h) reinterpret_cast<SparseConv3dLayerPlugin*>(h)
 #define H_S2D(h) reinterpret_cast<Sparse2DensePlugin*>(h)
+#define H_NORM(h) reinterpret_cast<RmsNormPlugin*>(h)
+#define H_LIN(h) reinterpret_cast<Linear8Plugin*>(h)
+#define H_ATT(h) reinterpret_cast<VoxelAttentionPlugin*>(h)
+#define CH_NORM(h) reinterpret_cast<const RmsNormPlugin*>(h)
+#define CH_LIN(h) reinterpret_cast<const Linear8Plugin*>(h)
+#define CH_ATT(h) reinterpret_cast<const VoxelAttentionPlugin*>(h)
 #define CH_VG(h) reinterpret_cast<const VoxelGeneratorPlugin*>(h)
 #define CH_SUBM(h) reinterpret_cast<const SubmConv3dLayerPlugin*>(h)
 #define CH_SP(h) reinterpret_cast<const SparseConv3dLayerPlugin*>(h)
@@ -285,5 +291,154 @@ int sessd_sparse2dense_set_padding(sessd_sparse2dense* h, int32_t top, int32_t b
     return H_S2D(h)->setPadding(top, bottom, left, right);
 }
 void sessd_sparse2dense_destroy(sessd_sparse2dense* h) { delete H_S2D(h); }
+
+// ------------------------------------------------------------------ rmsnorm
+int sessd_rmsnorm_create(const sessd_rmsnorm_desc* desc, const float* gamma, sessd_rmsnorm** out) {
+    NEED(desc && gamma && out, "null argument");
+    return guarded(__func__, [&]() -> int {
+        RmsNormPlugin* p = nullptr;
+        SESSD_TRY(RmsNormPlugin::create(*desc, gamma, &p));
+        *out = reinterpret_cast<sessd_rmsnorm*>(p);
+        return SESSD_OK;
+    });
+}
+int sessd_rmsnorm_deserialize(const void* bytes, size_t n, sessd_rmsnorm** out) {
+    NEED(out, "null argument");
+    return guarded(__func__, [&]() -> int {
+        RmsNormPlugin* p = nullptr;
+        SESSD_TRY(RmsNormPlugin::deserialize(bytes, n, &p));
+        *out = reinterpret_cast<sessd_rmsnorm*>(p);
+        return SESSD_OK;
+    });
+}
+size_t sessd_rmsnorm_serialization_size(const sessd_rmsnorm* h) { return h ? CH_NORM(h)->getSerializationSize() : 0; }
+int sessd_rmsnorm_serialize(const sessd_rmsnorm* h, void* buf) {
+    NEED(h && buf, "null argument");
+    CH_NORM(h)->serialize(buf);
+    return SESSD_OK;
+}
+int sessd_rmsnorm_configure(sessd_rmsnorm* h, const sessd_tensor_desc* in, int nIn, const sessd_tensor_desc* out, int nOut) {
+    NEED(h, "null handle");
+    return H_NORM(h)->configurePlugin(in, nIn, out, nOut);
+}
+size_t sessd_rmsnorm_workspace_size(const sessd_rmsnorm* h, const sessd_tensor_desc* in, int nIn, const sessd_tensor_desc* out,
+                                     int nOut) {
+    return h ? CH_NORM(h)->getWorkspaceSize(in, nIn, out, nOut) : 0;
+}
+int sessd_rmsnorm_enqueue(sessd_rmsnorm* h, const sessd_tensor_desc* inDesc, const sessd_tensor_desc* outDesc,
+                          const void* const* inputs, void* const* outputs, void* workspace, sessd_stream_t stream) {
+    NEED(h, "null handle");
+    return H_NORM(h)->enqueue(inDesc, outDesc, inputs, outputs, workspace, static_cast<hipStream_t>(stream));
+}
+int sessd_rmsnorm_set_flags(sessd_rmsnorm* h, int32_t flags) {
+    NEED(h, "null handle");
+    H_NORM(h)->flags_ = flags;
+    return SESSD_OK;
+}
+void sessd_rmsnorm_destroy(sessd_rmsnorm* h) { delete H_NORM(h); }
+
+// ------------------------------------------------------------------ linear8
+int sessd_linear8_create(const sessd_linear8_desc* desc, const float* weights, sessd_linear8** out) {
+    NEED(desc && weights && out, "null argument");
+    return guarded(__func__, [&]() -> int {
+        Linear8Plugin* p = nullptr;
+        SESSD_TRY(Linear8Plugin::create(*desc, weights, &p));
+        *out = reinterpret_cast<sessd_linear8*>(p);
+        return SESSD_OK;
+    });
+}
+int sessd_linear8_deserialize(const void* bytes, size_t n, sessd_linear8** out) {
+    NEED(out, "null argument");
+    return guarded(__func__, [&]() -> int {
+        Linear8Plugin* p = nullptr;
+        SESSD_TRY(Linear8Plugin::deserialize(bytes, n, &p));
+        *out = reinterpret_cast<sessd_linear8*>(p);
+        return SESSD_OK;
+    });
+}
+size_t sessd_linear8_serialization_size(const sessd_linear8* h) { return h ? CH_LIN(h)->getSerializationSize() : 0; }
+int sessd_linear8_serialize(const sessd_linear8* h, void* buf) {
+    NEED(h && buf, "null argument");
+    CH_LIN(h)->serialize(buf);
+    return SESSD_OK;
+}
+int sessd_linear8_configure(sessd_linear8* h, const sessd_tensor_desc* in, int nIn, const sessd_tensor_desc* out, int nOut) {
+    NEED(h, "null handle");
+    return H_LIN(h)->configurePlugin(in, nIn, out, nOut);
+}
+size_t sessd_linear8_workspace_size(const sessd_linear8* h, const sessd_tensor_desc* in, int nIn, const sessd_tensor_desc* out,
+                                     int nOut) {
+    return h ? CH_LIN(h)->getWorkspaceSize(in, nIn, out, nOut) : 0;
+}
+int sessd_linear8_enqueue(sessd_linear8* h, const sessd_tensor_desc* inDesc, const sessd_tensor_desc* outDesc,
+                          const void* const* inputs, void* const* outputs, void* workspace, sessd_stream_t stream) {
+    NEED(h, "null handle");
+    return H_LIN(h)->enqueue(inDesc, outDesc, inputs, outputs, workspace, static_cast<hipStream_t>(stream));
+}
+int sessd_linear8_set_epilogue(sessd_linear8* h, const float* scale, const float* shift, int relu) {
+    NEED(h, "null handle");
+    return guarded(__func__, [&]() -> int { return H_LIN(h)->setEpilogue(scale, shift, relu); });
+}
+int sessd_linear8_set_flags(sessd_linear8* h, int32_t flags) {
+    NEED(h, "null handle");
+    H_LIN(h)->flags_ = flags;
+    return SESSD_OK;
+}
+void sessd_linear8_destroy(sessd_linear8* h) { delete H_LIN(h); }
+
+// ------------------------------------------------------------------ voxelattn
+int sessd_voxelattn_create(const sessd_voxelattn_desc* desc, const float* slopes, sessd_voxelattn** out) {
+    NEED(desc && out, "null argument");
+    return guarded(__func__, [&]() -> int {
+        VoxelAttentionPlugin* p = nullptr;
+        SESSD_TRY(VoxelAttentionPlugin::create(*desc, slopes, &p));
+        *out = reinterpret_cast<sessd_voxelattn*>(p);
+        return SESSD_OK;
+    });
+}
+int sessd_voxelattn_deserialize(const void* bytes, size_t n, sessd_voxelattn** out) {
+    NEED(out, "null argument");
+    return guarded(__func__, [&]() -> int {
+        VoxelAttentionPlugin* p = nullptr;
+        SESSD_TRY(VoxelAttentionPlugin::deserialize(bytes, n, &p));
+        *out = reinterpret_cast<sessd_voxelattn*>(p);
+        return SESSD_OK;
+    });
+}
+size_t sessd_voxelattn_serialization_size(const sessd_voxelattn* h) { return h ? CH_ATT(h)->getSerializationSize() : 0; }
+int sessd_voxelattn_serialize(const sessd_voxelattn* h, void* buf) {
+    NEED(h && buf, "null argument");
+    CH_ATT(h)->serialize(buf);
+    return SESSD_OK;
+}
+int sessd_voxelattn_configure(sessd_voxelattn* h, const sessd_tensor_desc* in, int nIn, const sessd_tensor_desc* out, int nOut) {
+    NEED(h, "null handle");
+    return H_ATT(h)->configurePlugin(in, nIn, out, nOut);
+}
+size_t sessd_voxelattn_workspace_size(const sessd_voxelattn* h, const sessd_tensor_desc* in, int nIn, const sessd_tensor_desc* out,
+                                     int nOut) {
+    return h ? CH_ATT(h)->getWorkspaceSize(in, nIn, out, nOut) : 0;
+}
+int sessd_voxelattn_enqueue(sessd_voxelattn* h, const sessd_tensor_desc* inDesc, const sessd_tensor_desc* outDesc,
+                          const void* const* inputs, void* const* outputs, void* workspace, sessd_stream_t stream) {
+    NEED(h, "null handle");
+    return H_ATT(h)->enqueue(inDesc, outDesc, inputs, outputs, workspace, static_cast<hipStream_t>(stream));
+}
+int sessd_voxelattn_enqueue_shared(sessd_voxelattn* h, const sessd_tensor_desc* inDesc, const sessd_tensor_desc* outDesc,
+                                   const void* const* inputs, void* const* outputs, const void* window_workspace,
+                                   sessd_stream_t stream) {
+    NEED(h, "null handle");
+    return H_ATT(h)->enqueueShared(inDesc, outDesc, inputs, outputs, window_workspace, static_cast<hipStream_t>(stream));
+}
+int sessd_voxelattn_status(const sessd_voxelattn* h, const void* workspace, sessd_stream_t stream, int32_t* status) {
+    NEED(h && workspace && status, "null argument");
+    return read_status_word(workspace, CH_ATT(h)->statusOffset(), static_cast<hipStream_t>(stream), status);
+}
+int sessd_voxelattn_set_flags(sessd_voxelattn* h, int32_t flags) {
+    NEED(h, "null handle");
+    H_ATT(h)->flags_ = flags;
+    return SESSD_OK;
+}
+void sessd_voxelattn_destroy(sessd_voxelattn* h) { delete H_ATT(h); }
 
 }  // extern "C"

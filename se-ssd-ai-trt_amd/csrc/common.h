@@ -88,7 +88,7 @@ inline int ilog2(uint32_t pow2) {
 }
 inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-inline size_t dtype_size(int32_t t) { return t == SESSD_HALF ? 2 : 4; }
+inline size_t dtype_size(int32_t t) { return t == SESSD_FP8 ? 1 : t == SESSD_HALF ? 2 : 4; }
 
 constexpr uint32_t kEmpty = 0xFFFFFFFFu;
 

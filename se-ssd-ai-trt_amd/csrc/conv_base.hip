@@ -173,18 +173,23 @@ static void write_epilogue_trailer(char*& d, const Epilogue& e) {
     for (float v : e.scale_host) writeToBuffer<float>(d, v);
     for (float v : e.shift_host) writeToBuffer<float>(d, v);
 }
-int read_epilogue_trailer(const char* d, size_t remaining, ConvPluginBase* p) {
+int read_epilogue(const char* d, size_t remaining, int channels, Epilogue* e) {
     if (remaining == 0) return SESSD_OK;
     if (remaining < 4 * sizeof(int)) return fail(SESSD_E_INVALID, "conv: truncated epilogue trailer");
     if (readFromBuffer<int>(d) != kEpilogueMagic) return fail(SESSD_E_INVALID, "conv: unknown trailer");
-    const int relu = readFromBuffer<int>(d);
+    e->relu = readFromBuffer<int>(d);
     const int has_scale = readFromBuffer<int>(d), has_shift = readFromBuffer<int>(d);
-    const size_t need = (size_t)(has_scale + has_shift) * p->out_channel_ * sizeof(float);
+    const size_t need = (size_t)((has_scale ? 1 : 0) + (has_shift ? 1 : 0)) * channels * sizeof(float);
     if (remaining - 4 * sizeof(int) < need) return fail(SESSD_E_INVALID, "conv: truncated epilogue trailer");
-    std::vector<float> sc, sh;
-    if (has_scale) for (int i = 0; i < p->out_channel_; ++i) sc.push_back(readFromBuffer<float>(d));
-    if (has_shift) for (int i = 0; i < p->out_channel_; ++i) sh.push_back(readFromBuffer<float>(d));
-    return p->setEpilogue(has_scale ? sc.data() : nullptr, has_shift ? sh.data() : nullptr, relu);
+    if (has_scale) for (int i = 0; i < channels; ++i) e->scale_host.push_back(readFromBuffer<float>(d));
+    if (has_shift) for (int i = 0; i < channels; ++i) e->shift_host.push_back(readFromBuffer<float>(d));
+    return SESSD_OK;
+}
+int read_epilogue_trailer(const char* d, size_t remaining, ConvPluginBase* p) {
+    Epilogue e;
+    SESSD_TRY(read_epilogue(d, remaining, p->out_channel_, &e));
+    if (remaining == 0) return SESSD_OK;
+    return p->setEpilogue(e.scale_host.empty() ? nullptr : e.scale_host.data(), e.shift_host.empty() ? nullptr : e.shift_host.data(), e.relu);
 }
 size_t conv_epilogue_trailer_size(const Epilogue& e) { return epilogue_trailer_size(e); }
 void conv_write_epilogue_trailer(char*& d, const Epilogue& e) { write_epilogue_trailer(d, e); }

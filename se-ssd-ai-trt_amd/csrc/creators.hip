@@ -4,7 +4,7 @@
 // The reference has one creator class per plugin; each walks the field collection, picks the fields it knows by
 // name and calls the plugin's constructor (voxelGenerator.cu:618-701, submConv3dlayer.cu:732-878,
 // sparseConv3dlayer.cu:918-1079, sparse2Dense.cu:316-373).  Here one function does that for the four plugins of
-// the 3-D front end, keyed by the reference's plugin names.  Where the reference constructs a plugin from zeros
+// the 3-D front end, keyed by the reference's plugin names, and for this library's own layers.  Where the reference constructs a plugin from zeros
 // when a field is missing, this returns an error that names the field.
 #include <cstring>
 
@@ -36,6 +36,17 @@ const FieldSpec kSparseFields[] = {  // sparseConv3dlayer.cu:923-934 (3-vectors 
 const FieldSpec kDenseFields[] = {  // sparse2Dense.cu:321-322
     {"feature_map_size", SESSD_FIELD_INT32, 3}, {"feature_map_channel", SESSD_FIELD_INT32, 1}};
 
+// The layers without a counterpart in the reference: the fields are those of their descs.
+const FieldSpec kNormFields[] = {{"channel", SESSD_FIELD_INT32, 1}, {"max_voxels", SESSD_FIELD_INT32, 1}, {"eps", SESSD_FIELD_FLOAT32, 1},
+                                 {"gamma", SESSD_FIELD_FLOAT32, 0}};
+const FieldSpec kLinear8Fields[] = {{"in_channel", SESSD_FIELD_INT32, 1}, {"out_channel", SESSD_FIELD_INT32, 1},
+                                    {"max_voxels", SESSD_FIELD_INT32, 1}, {"weights", SESSD_FIELD_FLOAT32, 0}};
+const FieldSpec kAttentionFields[] = {
+    {"num_heads", SESSD_FIELD_INT32, 1},     {"num_kv_heads", SESSD_FIELD_INT32, 1}, {"head_dim", SESSD_FIELD_INT32, 1},
+    {"max_voxels", SESSD_FIELD_INT32, 1},    {"spatial_shape", SESSD_FIELD_INT32, 3}, {"window_shape", SESSD_FIELD_INT32, 3},
+    {"window_shift", SESSD_FIELD_INT32, 3},  {"cell_size", SESSD_FIELD_FLOAT32, 3},  {"softmax_scale", SESSD_FIELD_FLOAT32, 1},
+    {"score_cap", SESSD_FIELD_FLOAT32, 1},   {"slopes", SESSD_FIELD_FLOAT32, 0}};
+
 struct Registry {
     const char* plugin_name;
     const FieldSpec* specs;
@@ -57,10 +68,13 @@ Registry make_registry(const char* name, const FieldSpec (&specs)[N]) {
 }
 
 Registry* registry(const char* plugin_name) {
-    static Registry all[4] = {make_registry("VoxelGeneratorPlugin", kVoxelGenFields),
+    static Registry all[7] = {make_registry("VoxelGeneratorPlugin", kVoxelGenFields),
                               make_registry("SubmConv3dLayerPlugin", kSubmFields),
                               make_registry("SparseConv3dLayerPlugin", kSparseFields),
-                              make_registry("Sparse2DensePlugin", kDenseFields)};
+                              make_registry("Sparse2DensePlugin", kDenseFields),
+                              make_registry("RmsNormPlugin", kNormFields),
+                              make_registry("Linear8Plugin", kLinear8Fields),
+                              make_registry("VoxelAttentionPlugin", kAttentionFields)};
     if (!plugin_name) return nullptr;
     for (Registry& r : all)
         if (!std::strcmp(r.plugin_name, plugin_name)) {
@@ -110,12 +124,12 @@ int get_floats(const sessd_plugin_field_collection* fc, const Registry& r, const
 }
 
 // the `weights` field: FP32 [K][Cin][Cout]; a length other than 0 or 1 (the reference declares 1) must be the element count
-int get_weights(const sessd_plugin_field_collection* fc, const Registry& r, int64_t expect, const float** w) {
+int get_weights(const sessd_plugin_field_collection* fc, const Registry& r, int64_t expect, const float** w, const char* name = "weights") {
     const void* p = nullptr;
     int32_t length = 0;
-    SESSD_TRY(find_field(fc, r, "weights", &p, &length));
+    SESSD_TRY(find_field(fc, r, name, &p, &length));
     if (length > 1 && length != expect)
-        return fail(SESSD_E_INVALID, "%s: field 'weights' holds %d values, the layer shape needs %lld", r.plugin_name, length,
+        return fail(SESSD_E_INVALID, "%s: field '%s' holds %d values, the layer shape needs %lld", r.plugin_name, name, length,
                     (long long)expect);
     *w = static_cast<const float*>(p);
     return SESSD_OK;
@@ -140,6 +154,18 @@ static int clone_conv(const P* src, P** out) {
         delete p;
         return rc;
     }
+    *out = p;
+    return SESSD_OK;
+}
+
+template <typename P, typename F>
+static int clone_layer(const P* src, P** out, F&& more) {
+    std::vector<char> blob(src->getSerializationSize());
+    src->serialize(blob.data());
+    P* p = nullptr;
+    SESSD_TRY(P::deserialize(blob.data(), blob.size(), &p));
+    p->flags_ = src->flags_;
+    more(p);
     *out = p;
     return SESSD_OK;
 }
@@ -197,6 +223,43 @@ static int plugin_create_unguarded(const char* plugin_name, const sessd_plugin_f
         const float* w = nullptr;
         SESSD_TRY(get_weights(fc, r, (int64_t)d.in_channel * d.out_channel * d.ksize * d.ksize * d.ksize, &w));  // :866
         return sessd_submconv3d_create(&d, w, reinterpret_cast<sessd_submconv3d**>(handle));
+    }
+    if (r.specs == kNormFields) {
+        sessd_rmsnorm_desc d;
+        std::memset(&d, 0, sizeof(d));
+        SESSD_TRY(get_ints(fc, r, "channel", &d.channel, 1));
+        SESSD_TRY(get_ints(fc, r, "max_voxels", &d.max_voxels, 1));
+        SESSD_TRY(get_floats(fc, r, "eps", &d.eps, 1));
+        const float* gamma = nullptr;
+        SESSD_TRY(get_weights(fc, r, d.channel, &gamma, "gamma"));
+        return sessd_rmsnorm_create(&d, gamma, reinterpret_cast<sessd_rmsnorm**>(handle));
+    }
+    if (r.specs == kLinear8Fields) {
+        sessd_linear8_desc d;
+        std::memset(&d, 0, sizeof(d));
+        SESSD_TRY(get_ints(fc, r, "in_channel", &d.in_channel, 1));
+        SESSD_TRY(get_ints(fc, r, "out_channel", &d.out_channel, 1));
+        SESSD_TRY(get_ints(fc, r, "max_voxels", &d.max_voxels, 1));
+        const float* w = nullptr;
+        SESSD_TRY(get_weights(fc, r, (int64_t)d.in_channel * d.out_channel, &w));
+        return sessd_linear8_create(&d, w, reinterpret_cast<sessd_linear8**>(handle));
+    }
+    if (r.specs == kAttentionFields) {
+        sessd_voxelattn_desc d;
+        std::memset(&d, 0, sizeof(d));
+        SESSD_TRY(get_ints(fc, r, "num_heads", &d.num_heads, 1));
+        SESSD_TRY(get_ints(fc, r, "num_kv_heads", &d.num_kv_heads, 1));
+        SESSD_TRY(get_ints(fc, r, "head_dim", &d.head_dim, 1));
+        SESSD_TRY(get_ints(fc, r, "max_voxels", &d.max_voxels, 1));
+        SESSD_TRY(get_ints(fc, r, "spatial_shape", d.spatial_shape, 3));
+        SESSD_TRY(get_ints(fc, r, "window_shape", d.window_shape, 3));
+        SESSD_TRY(get_ints(fc, r, "window_shift", d.window_shift, 3));
+        SESSD_TRY(get_floats(fc, r, "cell_size", d.cell_size, 3));
+        SESSD_TRY(get_floats(fc, r, "softmax_scale", &d.softmax_scale, 1));
+        SESSD_TRY(get_floats(fc, r, "score_cap", &d.score_cap, 1));
+        const float* slopes = nullptr;
+        SESSD_TRY(get_weights(fc, r, d.num_heads, &slopes, "slopes"));
+        return sessd_voxelattn_create(&d, slopes, reinterpret_cast<sessd_voxelattn**>(handle));
     }
     sessd_sparseconv3d_desc d;
     std::memset(&d, 0, sizeof(d));
@@ -269,6 +332,33 @@ int sessd_sparse2dense_clone(const sessd_sparse2dense* h, sessd_sparse2dense** o
         p->out_type_ = src->out_type_;
         *out = reinterpret_cast<sessd_sparse2dense*>(p);
         return SESSD_OK;
+    });
+}
+
+int sessd_rmsnorm_clone(const sessd_rmsnorm* h, sessd_rmsnorm** out) {
+    if (!h || !out) return fail(SESSD_E_INVALID, "rmsnorm_clone: null argument");
+    return guarded(__func__, [&]() -> int {
+        const auto* src = reinterpret_cast<const RmsNormPlugin*>(h);
+        return clone_layer(src, reinterpret_cast<RmsNormPlugin**>(out), [&](RmsNormPlugin* p) {
+            p->type_ = src->type_;
+            p->residual_ = src->residual_;
+        });
+    });
+}
+
+int sessd_linear8_clone(const sessd_linear8* h, sessd_linear8** out) {
+    if (!h || !out) return fail(SESSD_E_INVALID, "linear8_clone: null argument");
+    return guarded(__func__, [&]() -> int {
+        const auto* src = reinterpret_cast<const Linear8Plugin*>(h);
+        return clone_layer(src, reinterpret_cast<Linear8Plugin**>(out), [&](Linear8Plugin* p) { p->out_type_ = src->out_type_; });
+    });
+}
+
+int sessd_voxelattn_clone(const sessd_voxelattn* h, sessd_voxelattn** out) {
+    if (!h || !out) return fail(SESSD_E_INVALID, "voxelattn_clone: null argument");
+    return guarded(__func__, [&]() -> int {
+        const auto* src = reinterpret_cast<const VoxelAttentionPlugin*>(h);
+        return clone_layer(src, reinterpret_cast<VoxelAttentionPlugin**>(out), [&](VoxelAttentionPlugin* p) { p->type_ = src->type_; });
     });
 }
 

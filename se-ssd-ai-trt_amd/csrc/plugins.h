@@ -1,8 +1,9 @@
-// plugins.h -- host classes behind the C-ABI.  One class per reference plugin, with the methods
+// plugins.h -- host classes behind the C-ABI.  One class per reference plugin, and one for each layer of this library's own, with the methods
 // TensorRT drives on IPluginV2DynamicExt (configurePlugin, getWorkspaceSize, enqueue,
 // getSerializationSize, serialize) under the same names; include/sessd3d.h forwards to them.
 #pragma once
 
+#include <memory>
 #include <vector>
 
 #include "coord.h"
@@ -275,6 +276,92 @@ class Sparse2DensePlugin {
     int in_type_ = SESSD_FLOAT, out_type_ = SESSD_FLOAT;
 };
 
+// ---------------------------------------------------------------------------------------------
+// Layers of a transformer block over voxel features; no counterpart in the reference
+// ---------------------------------------------------------------------------------------------
+class RmsNormPlugin {
+  public:
+    ~RmsNormPlugin();
+    static int create(const sessd_rmsnorm_desc& d, const float* gamma, RmsNormPlugin** out);
+    static int deserialize(const void* data, size_t length, RmsNormPlugin** out);
+    int configurePlugin(const sessd_tensor_desc* in, int nbInputs, const sessd_tensor_desc* out, int nbOutputs);
+    size_t getWorkspaceSize(const sessd_tensor_desc*, int, const sessd_tensor_desc*, int) const { return 0; }
+    int enqueue(const sessd_tensor_desc* inputDesc, const sessd_tensor_desc* outputDesc, const void* const* inputs,
+                void* const* outputs, void* workspace, hipStream_t stream);
+    size_t getSerializationSize() const;
+    void serialize(void* buffer) const;
+
+    int channel_ = 0, max_voxels_ = 0;
+    float eps_ = 0;
+    std::vector<float> gamma_;
+    float* gamma_dev_ = nullptr;
+    int type_ = SESSD_FLOAT;
+    bool residual_ = false;  // configured with a third input
+    int flags_ = 0;
+
+  private:
+    int check(const sessd_tensor_desc* in, const sessd_tensor_desc* out, bool residual) const;
+};
+
+class Linear8Plugin {
+  public:
+    ~Linear8Plugin();
+    static int create(const sessd_linear8_desc& d, const float* weights, Linear8Plugin** out);
+    static int deserialize(const void* data, size_t length, Linear8Plugin** out);
+    int setEpilogue(const float* scale, const float* shift, int relu);
+    int configurePlugin(const sessd_tensor_desc* in, int nbInputs, const sessd_tensor_desc* out, int nbOutputs);
+    size_t getWorkspaceSize(const sessd_tensor_desc*, int, const sessd_tensor_desc*, int) const { return 0; }
+    int enqueue(const sessd_tensor_desc* inputDesc, const sessd_tensor_desc* outputDesc, const void* const* inputs,
+                void* const* outputs, void* workspace, hipStream_t stream);
+    size_t getSerializationSize() const;
+    void serialize(void* buffer) const;
+
+    int in_channel_ = 0, out_channel_ = 0, max_voxels_ = 0;
+    std::vector<float> weights_;         // as given, FP32 [Cin][Cout]
+    __half* weights_packed_dev_ = nullptr;  // e4m3 values as halves, operand order (linear8.hip)
+    float* columns_dev_ = nullptr;       // wscale, scale, shift: three rows of out_channel_ floats, padded (linear8.hip)
+    Epilogue epi_;                       // (host side; the device has it in columns_dev_)
+    int out_type_ = SESSD_FLOAT;
+    int flags_ = 0;
+
+  private:
+    int check(const sessd_tensor_desc* in, const sessd_tensor_desc* out) const;
+    int uploadColumns();
+    std::vector<float> wscale_;
+};
+
+class VoxelAttentionPlugin {
+  public:
+    ~VoxelAttentionPlugin();
+    static int create(const sessd_voxelattn_desc& d, const float* slopes, VoxelAttentionPlugin** out);
+    static int deserialize(const void* data, size_t length, VoxelAttentionPlugin** out);
+    int configurePlugin(const sessd_tensor_desc* in, int nbInputs, const sessd_tensor_desc* out, int nbOutputs);
+    size_t getWorkspaceSize(const sessd_tensor_desc* in, int nbInputs, const sessd_tensor_desc* out, int nbOutputs) const;
+    int enqueue(const sessd_tensor_desc* inputDesc, const sessd_tensor_desc* outputDesc, const void* const* inputs,
+                void* const* outputs, void* workspace, hipStream_t stream);
+    int enqueueShared(const sessd_tensor_desc* inputDesc, const sessd_tensor_desc* outputDesc, const void* const* inputs,
+                      void* const* outputs, const void* window_workspace, hipStream_t stream);
+    size_t getSerializationSize() const;
+    void serialize(void* buffer) const;
+    size_t statusOffset() const { return 0; }
+
+    sessd_voxelattn_desc desc_ = {};
+    std::vector<float> slopes_;  // empty: no bias
+    float* slopes_dev_ = nullptr;
+    int type_ = SESSD_FLOAT;
+    int flags_ = 0;
+
+  private:
+    int check(const sessd_tensor_desc* in, const sessd_tensor_desc* out) const;
+    int checkCall(const sessd_tensor_desc* inputDesc, const sessd_tensor_desc* outputDesc, const void* const* inputs,
+                  void* const* outputs, const void* workspace, const char* who) const;
+    int attend(const void* const* inputs, void* const* outputs, const void* workspace, hipStream_t stream) const;
+};
+
+// Tensors of these layers: [1, max_voxels, channels]; the scalars in device memory
+int check_rows(const sessd_tensor_desc& d, int max_voxels, int channels, const char* who, const char* what);
+bool is_scalar_int(const sessd_tensor_desc& d);
+
 // little-endian field (de)serialisation in declaration order, as the reference's
 // writeToBuffer / readFromBuffer (voxelGenerator.cu:44-58)
 template <typename T>
@@ -298,6 +385,7 @@ int voxelgen_static_scratch(void** out);
 int conv_check_io(const sessd_tensor_desc* inputDesc, const sessd_tensor_desc* outputDesc,
                   const void* const* inputs, void* const* outputs, int in_type, int out_type, int max_voxels,
                   int cin, int cout, const char* who);
+int read_epilogue(const char* d, size_t remaining, int channels, Epilogue* e);
 int read_epilogue_trailer(const char* d, size_t remaining, ConvPluginBase* p);
 size_t conv_epilogue_trailer_size(const Epilogue& e);
 void conv_write_epilogue_trailer(char*& d, const Epilogue& e);

@@ -51,7 +51,8 @@ def lib():
     VPP = C.POINTER(C.c_void_p)
     L.sessd_last_error.restype = C.c_char_p
     L.sessd_version.restype = C.c_char_p
-    for name in ("voxelgen", "submconv3d", "sparseconv3d", "sparse2dense"):
+    plugins = ("voxelgen", "submconv3d", "sparseconv3d", "sparse2dense", "rmsnorm", "linear8", "voxelattn")
+    for name in plugins:
         getattr(L, "sessd_%s_serialization_size" % name).restype = sz
         getattr(L, "sessd_%s_serialization_size" % name).argtypes = [vp]
         getattr(L, "sessd_%s_serialize" % name).argtypes = [vp, vp]
@@ -62,11 +63,13 @@ def lib():
         getattr(L, "sessd_%s_enqueue" % name).argtypes = [vp, TD, TD, vp, vp, vp, vp]  # (pointer arrays: _pointers())
         getattr(L, "sessd_%s_destroy" % name).argtypes = [vp]
         getattr(L, "sessd_%s_destroy" % name).restype = None
-    for name in ("voxelgen", "submconv3d", "sparseconv3d"):
+    for name in ("voxelgen", "submconv3d", "sparseconv3d", "voxelattn"):
         getattr(L, "sessd_%s_status" % name).argtypes = [vp, vp, vp, C.POINTER(i32)]
+    for name in ("voxelgen", "submconv3d", "sparseconv3d", "rmsnorm", "linear8", "voxelattn"):
         getattr(L, "sessd_%s_set_flags" % name).argtypes = [vp, i32]
-    for name in ("submconv3d", "sparseconv3d"):
+    for name in ("submconv3d", "sparseconv3d", "linear8"):
         getattr(L, "sessd_%s_set_epilogue" % name).argtypes = [vp, vp, vp, C.c_int]
+    for name in ("submconv3d", "sparseconv3d"):
         getattr(L, "sessd_%s_export_rulebook" % name).argtypes = [vp, vp, vp, vp, vp]
     L.sessd_voxelgen_create.argtypes = [C.POINTER(D.VoxelGenDesc), VPP]
     L.sessd_voxelgen_grid_size.argtypes = [vp, C.POINTER(i32)]
@@ -75,6 +78,10 @@ def lib():
     L.sessd_submconv3d_enqueue_shared.argtypes = [vp, TD, TD, vp, vp, vp, vp]
     L.sessd_sparseconv3d_create.argtypes = [C.POINTER(D.SparseConv3dDesc), vp, VPP]
     L.sessd_sparse2dense_create.argtypes = [C.POINTER(D.Sparse2DenseDesc), VPP]
+    L.sessd_rmsnorm_create.argtypes = [C.POINTER(D.RmsNormDesc), vp, VPP]
+    L.sessd_linear8_create.argtypes = [C.POINTER(D.Linear8Desc), vp, VPP]
+    L.sessd_voxelattn_create.argtypes = [C.POINTER(D.VoxelAttnDesc), vp, VPP]
+    L.sessd_voxelattn_enqueue_shared.argtypes = [vp, TD, TD, vp, vp, vp, vp]
     L.sessd_sparse2dense_set_padding.argtypes = [C.c_void_p] + [C.c_int32] * 4
     L.sessd_sparse2dense_set_padding.restype = C.c_int
     FPP = C.POINTER(C.POINTER(C.c_float))
@@ -109,7 +116,7 @@ def lib():
     L.sessd_plugin_field_names.restype = C.POINTER(D.PluginFieldCollection)
     L.sessd_plugin_field_names.argtypes = [C.c_char_p]
     L.sessd_plugin_create.argtypes = [C.c_char_p, C.POINTER(D.PluginFieldCollection), VPP]
-    for name in ("voxelgen", "submconv3d", "sparseconv3d", "sparse2dense"):
+    for name in plugins:
         getattr(L, "sessd_%s_clone" % name).argtypes = [vp, VPP]
     _lib = L
     return L
@@ -156,7 +163,8 @@ def _np_f32_ptr(a):
 
 def _dtype_code(t):
     torch = _torch()
-    return {torch.float32: D.SESSD_FLOAT, torch.float16: D.SESSD_HALF, torch.int32: D.SESSD_INT32}[t.dtype]
+    return {torch.float32: D.SESSD_FLOAT, torch.float16: D.SESSD_HALF, torch.int32: D.SESSD_INT32,
+            torch.float8_e4m3fn: D.SESSD_FP8}[t.dtype]
 
 
 def _descs(tensors):
@@ -447,6 +455,92 @@ class Sparse2Dense(_Plugin):
         return int(self.ws[:4].view(torch.int32)[0].item())
 
 
+class RmsNorm(_Plugin):
+    """h = feat + residual; gamma * h / sqrt(mean(h^2) + eps) in e4m3 with a scale for each row."""
+    kind = "rmsnorm"
+
+    def __init__(self, channel, gamma, max_voxels=B.MAX_VOXELS, eps=1e-6):
+        d = D.RmsNormDesc(channel, max_voxels, eps)
+        g = np.ascontiguousarray(gamma, np.float32)
+        assert g.shape == (channel,)
+        h = C.c_void_p()
+        check(lib().sessd_rmsnorm_create(C.byref(d), _np_f32_ptr(g), C.byref(h)))
+        super().__init__(h)
+        self.max_voxels, self.channel = max_voxels, channel
+
+    def __call__(self, feat, voxel_num, residual=None, stream=None):
+        """feat, residual [max_voxels, channel] -> q float8_e4m3fn, scale f32 [max_voxels, 1] (, sum as feat, with a residual)"""
+        torch = _torch()
+        q = feat.new_empty((self.max_voxels, self.channel), dtype=torch.float8_e4m3fn)
+        scale = feat.new_empty((self.max_voxels, 1), dtype=torch.float32)
+        if residual is None:
+            ins, outs = (feat, voxel_num), (q, scale)
+        else:
+            ins, outs = (feat, voxel_num, residual), (q, scale, feat.new_empty((self.max_voxels, self.channel)))
+        self._enqueue_bound(self._bound_configured(ins, outs), ins, outs, stream)
+        return outs
+
+
+class Linear8(_Plugin):
+    """Rows in e4m3 times weights in e4m3, with the convolutions' epilogue."""
+    kind = "linear8"
+
+    def __init__(self, in_channel, out_channel, weights, max_voxels=B.MAX_VOXELS):
+        d = D.Linear8Desc(in_channel, out_channel, max_voxels)
+        w = np.ascontiguousarray(weights, np.float32)
+        assert w.shape == (in_channel, out_channel)
+        h = C.c_void_p()
+        check(lib().sessd_linear8_create(C.byref(d), _np_f32_ptr(w), C.byref(h)))
+        super().__init__(h)
+        self.max_voxels, self.cout = max_voxels, out_channel
+
+    def set_epilogue(self, scale=None, shift=None, relu=True):
+        sc = None if scale is None else np.ascontiguousarray(scale, np.float32)
+        sh = None if shift is None else np.ascontiguousarray(shift, np.float32)
+        assert all(v is None or v.shape == (self.cout,) for v in (sc, sh))
+        check(self._fn("set_epilogue")(self.h, _np_f32_ptr(sc), _np_f32_ptr(sh), int(relu)))
+
+    def __call__(self, q, scale, voxel_num, out_dtype=None, stream=None):
+        """q float8_e4m3fn [max_voxels, in_channel], scale f32 [max_voxels, 1] -> [max_voxels, out_channel], FP16 unless said otherwise"""
+        out = q.new_empty((self.max_voxels, self.cout), dtype=out_dtype or _torch().float16)
+        ins, outs = (q, scale, voxel_num), (out,)
+        self._enqueue_bound(self._bound_configured(ins, outs), ins, outs, stream)
+        return out
+
+
+class VoxelAttention(_Plugin):
+    """Attention among the voxels of a window of the grid: optional tanh cap of the scores, optional bias by distance."""
+    kind = "voxelattn"
+
+    def __init__(self, num_heads, num_kv_heads, head_dim, spatial_shape_xyz, window_xyz, shift_xyz=(0, 0, 0), slopes=None,
+                 cell_size_xyz=(1.0, 1.0, 1.0), cap=0.0, softmax_scale=0.0, max_voxels=B.MAX_VOXELS):
+        d = D.VoxelAttnDesc()
+        d.num_heads, d.num_kv_heads, d.head_dim, d.max_voxels = num_heads, num_kv_heads, head_dim, max_voxels
+        for a in range(3):
+            d.spatial_shape[a], d.window_shape[a], d.window_shift[a] = spatial_shape_xyz[a], window_xyz[a], shift_xyz[a]
+            d.cell_size[a] = cell_size_xyz[a]
+        d.softmax_scale, d.score_cap = softmax_scale, cap
+        s = None if slopes is None else np.ascontiguousarray(slopes, np.float32)
+        assert s is None or s.shape == (num_heads,)
+        h = C.c_void_p()
+        check(lib().sessd_voxelattn_create(C.byref(d), _np_f32_ptr(s), C.byref(h)))
+        super().__init__(h)
+        self.max_voxels, self.cout = max_voxels, num_heads * head_dim
+
+    def __call__(self, qkv, coors, voxel_num, stream=None, windows_from=None):
+        """qkv [max_voxels, (num_heads + 2 num_kv_heads) * head_dim] -> [max_voxels, num_heads * head_dim].  windows_from: a layer on
+        the same coordinates and windows that has run on this stream."""
+        out = qkv.new_empty((self.max_voxels, self.cout))
+        ins, outs = (qkv, coors, voxel_num), (out,)
+        bound = self._bound_configured(ins, outs)
+        if windows_from is None:
+            self._enqueue_bound(bound, ins, outs, stream)
+        else:
+            check(lib().sessd_voxelattn_enqueue_shared(self.h, bound.ins, bound.outs, _pointers(ins), _pointers(outs),
+                                                       _ptr(windows_from.ws), _stream_ptr(stream)))
+        return out
+
+
 PLUGIN_CLASSES = {}
 
 
@@ -475,7 +569,8 @@ def create_plugin(plugin_name, fields):
     h = C.c_void_p()
     check(lib().sessd_plugin_create(plugin_name.encode(), C.byref(fc), C.byref(h)))
     cls = {"VoxelGeneratorPlugin": VoxelGenerator, "SubmConv3dLayerPlugin": SubmConv3d,
-           "SparseConv3dLayerPlugin": SparseConv3d, "Sparse2DensePlugin": Sparse2Dense}[plugin_name]
+           "SparseConv3dLayerPlugin": SparseConv3d, "Sparse2DensePlugin": Sparse2Dense,
+           "RmsNormPlugin": RmsNorm, "Linear8Plugin": Linear8, "VoxelAttentionPlugin": VoxelAttention}[plugin_name]
     obj = cls.__new__(cls)
     _Plugin.__init__(obj, h)
     g = lambda k: np.asarray(fields[k]).reshape(-1)  # noqa: E731
@@ -483,6 +578,12 @@ def create_plugin(plugin_name, fields):
         obj.max_voxels = int(g("max_voxels")[0])
     elif cls is Sparse2Dense:
         obj.size, obj.channel, obj.padding = tuple(int(v) for v in g("feature_map_size")), int(g("feature_map_channel")[0]), (0, 0, 0, 0)
+    elif cls is RmsNorm:
+        obj.max_voxels, obj.channel = int(g("max_voxels")[0]), int(g("channel")[0])
+    elif cls is Linear8:
+        obj.max_voxels, obj.cout = int(g("max_voxels")[0]), int(g("out_channel")[0])
+    elif cls is VoxelAttention:
+        obj.max_voxels, obj.cout = int(g("max_voxels")[0]), int(g("num_heads")[0]) * int(g("head_dim")[0])
     else:
         obj.max_voxels, obj.cout = int(g("max_voxels")[0]), int(g("out_channel")[0])
         k = g("ksize")

@@ -4,6 +4,7 @@ import ctypes as C
 SESSD_FLOAT = 0
 SESSD_HALF = 1
 SESSD_INT32 = 3
+SESSD_FP8 = 6
 
 SESSD_OK = 0
 SESSD_E_INVALID = 1
@@ -61,6 +62,20 @@ class SparseConv3dDesc(C.Structure):
 
 class Sparse2DenseDesc(C.Structure):
     _fields_ = [("feature_map_size", C.c_int32 * 3), ("feature_map_channel", C.c_int32)]
+
+
+class RmsNormDesc(C.Structure):
+    _fields_ = [("channel", C.c_int32), ("max_voxels", C.c_int32), ("eps", C.c_float)]
+
+
+class Linear8Desc(C.Structure):
+    _fields_ = [("in_channel", C.c_int32), ("out_channel", C.c_int32), ("max_voxels", C.c_int32)]
+
+
+class VoxelAttnDesc(C.Structure):
+    _fields_ = [("num_heads", C.c_int32), ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("max_voxels", C.c_int32),
+                ("spatial_shape", C.c_int32 * 3), ("window_shape", C.c_int32 * 3), ("window_shift", C.c_int32 * 3),
+                ("cell_size", C.c_float * 3), ("softmax_scale", C.c_float), ("score_cap", C.c_float)]
 
 
 class LayerSpec(C.Structure):
