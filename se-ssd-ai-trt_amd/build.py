@@ -26,7 +26,8 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-fast-math"
 
 # conv_tile.hip keeps its accumulators over a loop in which nothing else may wait; left to itself the compiler puts them
 # into accumulation registers and copies them back and forth once per kernel offset
-FILE_FLAGS = {"conv_tile.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+# (voxel_attention.h's as well)
+FILE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("conv_tile.hip", "voxel_attention.hip", "voxel_attention_f32.hip")}
 
 
 def sources():

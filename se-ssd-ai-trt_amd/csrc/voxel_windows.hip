@@ -1,0 +1,208 @@
+// voxel_windows.hip -- the rows of a sparse tensor, which come in the order in which their voxels were met, by the windows of a grid.
+//
+// A window's rows are listed ascending, so that the order of a row's sums does not depend on chance; where a window's rows begin does.
+//
+//   window_count   1 024 rows a workgroup: each row's place among its window's rows of the chunk, and the chunk's counts for all windows.
+//                  A wave finds the lanes that share a window with ballots over the window's bits; then the waves add their counts one
+//                  after the other, in LDS
+//   window_base    a thread for each window: its rows over all chunks, its place in the list, each chunk's place in it, its work items
+//   window_place   rows into the list
+//
+// No atomics in the first pass: all of a near window's rows would ask at one address, 24 ns each (627 rows of 16 000 in one window: 15 us).
+// Where a window count is beyond what LDS holds (kMostCounted), windows are small and tickets are given out by atomics:
+//
+//   window_ticket, window_base, window_scatter, window_rank    the last puts a window's rows in ascending order
+#include "fill.h"
+#include "voxel_windows.h"
+
+namespace sessd {
+
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kChunk = 1024;
+constexpr int kMostCounted = 32768;  // windows: 64 KB of 16-bit counts
+constexpr int kLong = 128;           // rows of a window whose items come first: the last to end should not be the last to begin
+
+size_t counted_windows(size_t windows) { return (windows + 7) / 8 * 8; }
+
+// window of a row's voxel, -1 = outside the grid
+__device__ __forceinline__ int window_of(const int4 c, const WindowGrid& g) {  // (b,z,y,x)
+    if (c.x != 0 || c.y < 0 || c.y >= g.shape[0] || c.z < 0 || c.z >= g.shape[1] || c.w < 0 || c.w >= g.shape[2]) return -1;
+    return ((c.y + g.shift[0]) / g.window[0] * g.count[1] + (c.z + g.shift[1]) / g.window[1]) * g.count[2] + (c.w + g.shift[2]) / g.window[2];
+}
+
+__global__ void __launch_bounds__(kChunk)
+window_count(const int32_t* __restrict__ coors, const int32_t* __restrict__ voxel_num, WindowGrid g, int windows, int bits, WindowIndex w) {
+    extern __shared__ uint4 s_count4[];
+    uint16_t* s_count = reinterpret_cast<uint16_t*>(s_count4);
+    const int row = blockIdx.x * kChunk + threadIdx.x, wave = threadIdx.x >> 6;
+    int4 c = make_int4(-1, 0, 0, 0);
+    if (row < w.max_voxels) c = reinterpret_cast<const int4*>(coors)[row];
+    for (int i = threadIdx.x; i < windows / 8; i += kChunk) s_count4[i] = make_uint4(0, 0, 0, 0);
+    if (blockIdx.x == 0 && threadIdx.x < kHeadWords) w.head[threadIdx.x] = 0;
+    const int n = clamp_rows(voxel_num, w.max_voxels);
+    if ((int)blockIdx.x * kChunk >= n) return;
+    const int key = row < n ? window_of(c, g) : -1;
+    uint64_t same = __ballot(key >= 0);
+    for (int b = 0; b < bits; ++b) {
+        const bool mine = (key >> b) & 1;
+        const uint64_t set = __ballot(mine);
+        same &= mine ? set : ~set;
+    }
+    const int rank = (int)rank_in_wave(same), group = (int)__popcll(same);
+    const int left = (n - (int)blockIdx.x * kChunk + 63) / 64, waves = left < kChunk / 64 ? left : kChunk / 64;
+    int before = 0;
+    __syncthreads();
+    for (int i = 0; i < waves; ++i) {
+        if (wave == i && key >= 0) {
+            before = s_count[key];
+            if (rank == group - 1) s_count[key] = (uint16_t)(before + group);
+        }
+        __syncthreads();
+    }
+    if (row < n) w.ticket[row] = make_int2(key, before + rank);
+    uint4* dst = reinterpret_cast<uint4*>(w.chunk_count + (size_t)blockIdx.x * windows);
+    for (int i = threadIdx.x; i < windows / 8; i += kChunk) dst[i] = s_count4[i];
+}
+
+// place `mine` of this lane behind those of the lanes before it, in a range of the list that the wave takes
+__device__ __forceinline__ int take(int32_t* from, int mine) {
+    const uint32_t upto = wave_scan((uint32_t)mine);
+    int at = 0;
+    if (lane_id() == 63 && upto) at = atomicAdd(from, (int)upto);
+    return __shfl(at, 63) + (int)upto - mine;
+}
+
+// chunks 0: the counts are w.count's, and the bases go to w.base
+__global__ void __launch_bounds__(kBlock)
+window_base(const int32_t* __restrict__ voxel_num, int windows, int chunked, WindowIndex w) {
+    const int i = blockIdx.x * kBlock + threadIdx.x;
+    const int chunks = chunked ? (clamp_rows(voxel_num, w.max_voxels) + kChunk - 1) / kChunk : 0;
+    int rows = 0;
+    if (i < windows) {
+        if (chunked) {
+#pragma unroll 8
+            for (int c = 0; c < chunks; ++c) rows += w.chunk_count[(size_t)c * windows + i];
+        } else {
+            rows = w.count[i];
+        }
+    }
+    const int base = take(&w.head[kHeadPlaces], rows);
+    const int items = (rows + kItemRows - 1) / kItemRows;
+    const bool is_long = rows > kLong;
+    const int front = take(&w.head[kHeadLong], is_long ? items : 0), back = take(&w.head[kHeadShort], is_long ? 0 : items);
+    if (!rows) return;
+    if (chunked) {
+        int at = base;
+#pragma unroll 8
+        for (int c = 0; c < chunks; ++c) {
+            w.chunk_base[(size_t)c * windows + i] = at;
+            at += w.chunk_count[(size_t)c * windows + i];
+        }
+    } else {
+        w.base[i] = base;
+    }
+    for (int k = 0; k < items; ++k) w.items[is_long ? front + k : w.items_cap - 1 - (back + k)] = make_int4(base, rows, k * kItemRows, 0);
+}
+
+__device__ __forceinline__ void set_place(const WindowIndex& w, int place, int row, const int4 c) {
+    w.order[place] = row;
+    w.cell[place] = make_float4((float)c.w, (float)c.z, (float)c.y, 0.f);
+}
+__device__ __forceinline__ void set_outside(const WindowIndex& w, int n, int row) {
+    w.order[n - 1 - atomicAdd(&w.head[kHeadOutside], 1)] = row;
+    atomicOr(&w.head[kHeadStatus], SESSD_STATUS_BAD_COORD);
+}
+
+__global__ void __launch_bounds__(kBlock)
+window_place(const int32_t* __restrict__ coors, const int32_t* __restrict__ voxel_num, int windows, WindowIndex w) {
+    const int row = blockIdx.x * kBlock + threadIdx.x;
+    if (row >= w.max_voxels) return;
+    const int4 c = reinterpret_cast<const int4*>(coors)[row];
+    const int n = clamp_rows(voxel_num, w.max_voxels);
+    if (row >= n) return;
+    const int2 t = w.ticket[row];
+    if (t.x >= 0) set_place(w, w.chunk_base[(size_t)(row / kChunk) * windows + t.x] + t.y, row, c);
+    else set_outside(w, n, row);
+}
+
+__global__ void __launch_bounds__(kBlock)
+window_ticket(const int32_t* __restrict__ coors, const int32_t* __restrict__ voxel_num, WindowGrid g, WindowIndex w) {
+    const int row = blockIdx.x * kBlock + threadIdx.x;
+    const int n = clamp_rows(voxel_num, w.max_voxels);
+    if (row >= n) return;
+    const int key = window_of(reinterpret_cast<const int4*>(coors)[row], g);
+    if (key < 0) set_outside(w, n, row);
+    w.ticket[row] = make_int2(key, key < 0 ? 0 : atomicAdd(&w.count[key], 1));
+}
+
+__global__ void __launch_bounds__(kBlock)
+window_scatter(const int32_t* __restrict__ voxel_num, WindowIndex w) {
+    const int row = blockIdx.x * kBlock + threadIdx.x;
+    if (row >= clamp_rows(voxel_num, w.max_voxels)) return;
+    const int2 t = w.ticket[row];
+    if (t.x >= 0) w.list[w.base[t.x] + t.y] = row;
+}
+
+__global__ void __launch_bounds__(kBlock)
+window_rank(const int32_t* __restrict__ coors, WindowIndex w) {
+    const int p = blockIdx.x * kBlock + threadIdx.x;
+    if (p >= w.head[kHeadPlaces]) return;
+    const int row = w.list[p], key = w.ticket[row].x;
+    const int start = w.base[key], rows = w.count[key];
+    int rank = 0;
+#pragma unroll 4
+    for (int i = 0; i < rows; ++i) rank += w.list[start + i] < row ? 1 : 0;
+    set_place(w, start + rank, row, reinterpret_cast<const int4*>(coors)[row]);
+}
+
+}  // namespace
+
+WindowIndex carve_windows(void* workspace, int max_voxels, size_t windows) {
+    const bool counted = windows <= kMostCounted;
+    const size_t rows = (size_t)max_voxels, chunks = (rows + kChunk - 1) / kChunk;
+    WorkspaceCarver c(workspace);
+    WindowIndex w;
+    w.max_voxels = max_voxels;
+    w.items_cap = (int32_t)((rows < windows ? rows : windows) + rows / kItemRows);
+    w.head = c.take<int32_t>(kHeadWords);
+    w.order = c.take<int32_t>(rows);
+    w.cell = c.take<float4>(rows);
+    w.items = c.take<int4>((size_t)w.items_cap);
+    w.ticket = c.take<int2>(rows);
+    w.chunk_count = c.take<uint16_t>(counted ? chunks * counted_windows(windows) : 0);
+    w.chunk_base = c.take<int32_t>(counted ? chunks * counted_windows(windows) : 0);
+    w.list = c.take<int32_t>(counted ? 0 : rows);
+    w.count = c.take<int32_t>(counted ? 0 : windows);
+    w.base = c.take<int32_t>(counted ? 0 : windows);
+    w.bytes = c.total();
+    return w;
+}
+
+int launch_windows(const int32_t* coors, const int32_t* voxel_num, const WindowGrid& g, const WindowIndex& w, hipStream_t stream) {
+    const dim3 rows((unsigned)ceil_div(w.max_voxels, kBlock)), block(kBlock);
+    if (g.windows() <= kMostCounted) {
+        const int windows = (int)counted_windows(g.windows());
+        int bits = 0;
+        while (((size_t)1 << bits) < g.windows()) ++bits;
+        hipLaunchKernelGGL(window_count, dim3((unsigned)ceil_div(w.max_voxels, kChunk)), dim3(kChunk), (size_t)windows * sizeof(uint16_t), stream, coors,
+                           voxel_num, g, windows, bits, w);
+        hipLaunchKernelGGL(window_base, dim3((unsigned)ceil_div(windows, kBlock)), block, 0, stream, voxel_num, windows, 1, w);
+        hipLaunchKernelGGL(window_place, rows, block, 0, stream, coors, voxel_num, windows, w);
+    } else {
+        const int windows = (int)g.windows();
+        FillArgs f;
+        f.add(w.head, kHeadWords, 0);
+        f.add(w.count, (uint64_t)windows, 0);
+        SESSD_TRY(launch_fill(f, stream));
+        hipLaunchKernelGGL(window_ticket, rows, block, 0, stream, coors, voxel_num, g, w);
+        hipLaunchKernelGGL(window_base, dim3((unsigned)ceil_div(windows, kBlock)), block, 0, stream, voxel_num, windows, 0, w);
+        hipLaunchKernelGGL(window_scatter, rows, block, 0, stream, voxel_num, w);
+        hipLaunchKernelGGL(window_rank, rows, block, 0, stream, coors, w);
+    }
+    SESSD_HIP_TRY(hipGetLastError());
+    return SESSD_OK;
+}
+
+}  // namespace sessd
