@@ -5,9 +5,14 @@
 // An e4m3 value is a half, so the rows are widened in registers (the weights at create) and multiplied by the FP16 matrix
 // instructions: products are exact, sums FP32, and one rounding to the output's type follows the epilogue.  The 8-bit matrix
 // instructions add with fewer bits: 512 -> 128 channels were 1.4e-5 of the result's norm from the 64-bit sums, 5e-8 these.
-// The product is taken transposed, D = Wq^T Q^T: a lane of the result has one row and, with the weights'
-// columns dealt to the instructions as they are, 16 neighbouring columns of it, which it stores as whole 16-byte words.
-// What bounds the layer at this library's widths is the output it writes.
+// The product is taken transposed, D = Wq^T Q^T: a lane of the result has one row and, with the weights' columns dealt to the
+// instructions as they are, 8 or 16 neighbouring columns of it, which it stores as whole 16-byte words.
+//
+// Up to kMostHeld input channels a wave keeps the weights of its columns (64, or 32 where the channels are many) in registers, 128 of
+// them at most, and takes one block of 16 rows after the other, the next one's values requested while it multiplies: nothing of the
+// weights is read twice, nothing goes through LDS but the epilogue's constants, and no wave waits for another.  The waves of a
+// workgroup have neighbouring columns of the same rows.  What bounds it then is the output it writes.  Wider inputs read the
+// weights anew for every 16 rows.
 #include <cmath>
 
 #include "plugins.h"
@@ -17,95 +22,176 @@ namespace sessd {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kColumns = 64;  // of a wave: four instructions, 16 each
-constexpr int kRows = 16;     // of a wave
-constexpr int kStep = 32;     // values of k to an instruction
+constexpr int kRows = 16;      // of a wave at a time
+constexpr int kMostHeld = 512;
+constexpr int kGroups = 512;   // workgroups of the kernel that holds its weights: two for each compute unit
+
+// instructions, 16 columns each, of a wave: as many as leave the held weights 128 registers
+constexpr int tiles_of(int cin) { return cin > 256 && cin <= kMostHeld ? 2 : 4; }
+// Rows and weights meet in 64 input channels at a time, two instructions: lane group g has 16 neighbouring channels of each row, 8 to either
+constexpr int pairs_of(int cin) { return (cin + 63) / 64; }
+constexpr int channel_of(int step, int g, int e) { return step / 2 * 64 + g * 16 + step % 2 * 8 + e; }
+// column that row `i` of instruction `t` stands for: lane group g (rows 4 g .. 4 g + 3) gets 4 NT neighbouring ones over the NT
+constexpr int column_of(int tiles, int t, int i) { return 4 * tiles * (i / 4) + 4 * t + i % 4; }
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef unsigned int v2u __attribute__((ext_vector_type(2)));
+typedef unsigned int v4u __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ v8h widen(v2u x) {
-    const v2h a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[0], 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[0], 1.f, true);
-    const v2h c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[1], 1.f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[1], 1.f, true);
+__device__ __forceinline__ v8h widen(unsigned x, unsigned y) {
+    const v2h a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.f, true);
+    const v2h c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y, 1.f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(y, 1.f, true);
     return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// column of the 64 that row `i` of instruction `t` stands for: lane group g (rows 4g .. 4g + 3) gets 16g .. 16g + 15 over the four
-__host__ __device__ constexpr int column_of(int t, int i) { return 16 * (i / 4) + 4 * t + i % 4; }
+struct LinearArgs {
+    const uint8_t* q;
+    const float* scale;
+    const int32_t* voxel_num;
+    int max_voxels, cin, cout, relu, write_pad;
+    const __half* w;       // [block of columns][step][instruction][lane][8]
+    const float* columns;  // of the result: factor, addend; two rows of whole blocks
+    void* out;
+};
 
-template <typename T>
-__device__ __forceinline__ void store_columns(T* dst, const float (&v)[16], int left, bool wide) {
-    if (wide && left >= 16) {
-        if constexpr (sizeof(T) == 2) {
+// 4 NT neighbouring columns of a row, from `c0` on
+template <typename T, int NT>
+__device__ __forceinline__ void store_columns(const LinearArgs& a, int row, int c0, const v4f (&acc)[NT], float s, const v4f* factor, const v4f* addend) {
+    float y[4 * NT];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+    for (int t = 0; t < NT; ++t) {
+        const v4f f = factor[t], b = addend[t];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float x = fmaf(acc[t][e] * s, f[e], b[e]);
+            y[4 * t + e] = a.relu && x < 0.f ? 0.f : x;
+        }
+    }
+    T* dst = static_cast<T*>(a.out) + (size_t)row * a.cout + c0;
+    constexpr int kPer = 16 / (int)sizeof(T);
+    if (a.cout % kPer == 0 && c0 + 4 * NT <= a.cout) {
+#pragma unroll
+        for (int i = 0; i < 4 * NT / kPer; ++i) {
+            if constexpr (sizeof(T) == 2) {
                 v8h x;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = (_Float16)v[8 * h + e];
-                reinterpret_cast<v8h*>(dst)[h] = x;
-            }
-        } else {
-#pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                v4f x;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = v[4 * h + e];
-                reinterpret_cast<v4f*>(dst)[h] = x;
+                for (int e = 0; e < 8; ++e) x[e] = (_Float16)y[8 * i + e];
+                reinterpret_cast<v8h*>(dst)[i] = x;
+            } else {
+                reinterpret_cast<v4f*>(dst)[i] = v4f{y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]};
             }
         }
-        return;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4 * NT; ++e)
+            if (c0 + e < a.cout) {
+                if constexpr (sizeof(T) == 2) dst[e] = __float2half_rn(y[e]);
+                else dst[e] = y[e];
+            }
     }
+}
+
+// PAIRS: of 64 input channels
+template <typename T, int PAIRS, int NT>
+__global__ void __launch_bounds__(kBlock, 2)
+linear8_held(LinearArgs a) {
+    constexpr int kWide = 16 * NT;
+    __shared__ v4f s_columns[kBlock / 64][2][kWide / 4];
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
+    const int blocks = (a.cout + kWide - 1) / kWide, id = (int)blockIdx.x * (kBlock / 64) + wave;
+    const int cb = id % blocks, stream = id / blocks, streams = (int)gridDim.x * (kBlock / 64) / blocks;
+    if (stream >= streams) return;  // (what is left over; no wave waits for another)
+    const int pairs = (a.cin + 63) / 64;
+    v8h w[2 * PAIRS][NT];
+    const v8h* from = reinterpret_cast<const v8h*>(a.w) + (size_t)cb * 2 * pairs * NT * 64 + lane;
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-        if (e < left) {
-            if constexpr (sizeof(T) == 2) dst[e] = __float2half_rn(v[e]);
-            else dst[e] = v[e];
+    for (int s = 0; s < 2 * PAIRS; ++s)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            if (s < 2 * pairs) w[s][t] = from[(s * NT + t) * 64];
+    if (lane < kWide / 4)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) s_columns[wave][i][lane] = reinterpret_cast<const v4f*>(a.columns + i * blocks * kWide + cb * kWide)[lane];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const int n = clamp_rows(a.voxel_num, a.max_voxels), rows = a.write_pad ? a.max_voxels : n;
+    v4u x[PAIRS];
+    float scale = 0.f;
+    const auto request = [&](int row) {  // a row's values, zeros behind the last one
+        scale = 0.f;
+        if (row < n) scale = a.scale[row];
+#pragma unroll
+        for (int p = 0; p < PAIRS; ++p) {
+            x[p] = v4u{0, 0, 0, 0};
+            if (row < n && p * 64 + g * 16 < a.cin) x[p] = *reinterpret_cast<const v4u*>(a.q + (size_t)row * a.cin + p * 64 + g * 16);
         }
+    };
+    request(stream * kRows + r);
+    for (int row0 = stream * kRows; row0 < rows; row0 += streams * kRows) {
+        v8h b[2 * PAIRS];
+#pragma unroll
+        for (int p = 0; p < PAIRS; ++p) {
+            b[2 * p] = widen(x[p][0], x[p][1]);
+            b[2 * p + 1] = widen(x[p][2], x[p][3]);
+        }
+        const float s = scale;
+        request(row0 + streams * kRows + r);
+        v4f acc[NT] = {};
+#pragma unroll
+        for (int k = 0; k < 2 * PAIRS; ++k)
+            if (k < 2 * pairs) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[k][t], b[k], acc[t], 0, 0, 0);
+            }
+        if (row0 + r < rows) store_columns<T, NT>(a, row0 + r, cb * kWide + 4 * NT * g, acc, s, s_columns[wave][0] + NT * g, s_columns[wave][1] + NT * g);
+    }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kBlock)
-linear8(const uint8_t* __restrict__ q, const float* __restrict__ scale, const int32_t* __restrict__ voxel_num, int max_voxels,
-        int cin, int cout, const __half* __restrict__ w, const float* __restrict__ columns, int cout_pad, int relu,
-        T* __restrict__ out, int write_pad) {
+linear8_wide(LinearArgs a) {
+    constexpr int NT = 4, kWide = 16 * NT;
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const int row = (blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6)) * kRows + r;
-    const int n = clamp_rows(voxel_num, max_voxels);
-    const int cb = blockIdx.y;
-    const int steps = (cin + kStep - 1) / kStep;
-    const bool active = row < n;
-    v4f acc[4] = {};
-    const __half* wp = w + ((size_t)cb * steps * 4 * 64 + lane) * 8;
-    const uint8_t* qp = q + (size_t)row * cin + g * 8;
-    for (int ks = 0; ks < steps; ++ks) {
-        v2u x = {};
-        if (active && ks * kStep + g * 8 < cin) x = *reinterpret_cast<const v2u*>(qp + ks * kStep);
-        const v8h b = widen(x);
+    const int row = ((int)blockIdx.x * (kBlock / 64) + (int)(threadIdx.x >> 6)) * kRows + r;
+    const int n = clamp_rows(a.voxel_num, a.max_voxels), cb = blockIdx.y, blocks = gridDim.y, pairs = (a.cin + 63) / 64;
+    v4f acc[NT] = {};
+    const v8h* w = reinterpret_cast<const v8h*>(a.w) + (size_t)cb * 2 * pairs * NT * 64 + lane;
+    for (int p = 0; p < pairs; ++p) {
+        v4u x = {0, 0, 0, 0};
+        if (row < n && p * 64 + g * 16 < a.cin) x = *reinterpret_cast<const v4u*>(a.q + (size_t)row * a.cin + p * 64 + g * 16);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const v8h a = *reinterpret_cast<const v8h*>(wp + (size_t)(ks * 4 + t) * 64 * 8);
-            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, acc[t], 0, 0, 0);
+        for (int h = 0; h < 2; ++h) {
+            const v8h b = widen(x[2 * h], x[2 * h + 1]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[((2 * p + h) * NT + t) * 64], b, acc[t], 0, 0, 0);
         }
     }
-    if (row >= max_voxels || (!active && !write_pad)) return;
-    const float s = active ? scale[row] : 0.f;
-    const int c0 = cb * kColumns + 16 * g;
-    if (c0 >= cout) return;
-    const v4f* col = reinterpret_cast<const v4f*>(columns + c0);
-    float v[16];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const v4f ws = col[t], sc = col[cout_pad / 4 + t], sh = col[cout_pad / 2 + t];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float y = acc[t][e] * s * ws[e] * sc[e] + sh[e];
-            if (relu) y = y < 0.f ? 0.f : y;
-            v[4 * t + e] = y;
-        }
+    if (row >= a.max_voxels || (row >= n && !a.write_pad)) return;
+    const int c0 = cb * kWide + 4 * NT * g;
+    const v4f* columns = reinterpret_cast<const v4f*>(a.columns + c0);
+    store_columns<T, NT>(a, row, c0, acc, row < n ? a.scale[row] : 0.f, columns, columns + blocks * kWide / 4);
+}
+
+template <typename T>
+void launch_linear8(const LinearArgs& a, hipStream_t stream) {
+    const int rows16 = ceil_div(a.max_voxels, kRows), blocks = ceil_div(a.cout, 16 * tiles_of(a.cin));
+    if (a.cin > kMostHeld) {
+        hipLaunchKernelGGL(linear8_wide<T>, dim3((unsigned)ceil_div(rows16, kBlock / 64), (unsigned)blocks), dim3(kBlock), 0, stream, a);
+        return;
     }
-    store_columns(out + (size_t)row * cout + c0, v, cout - c0, cout % (16 / (int)sizeof(T)) == 0);
+    // (at least a wave for each block of columns)
+    const int64_t most = ceil_div((int64_t)rows16 * blocks, kBlock / 64);
+    const int groups = most < kGroups ? (int)most : kGroups > ceil_div(blocks, kBlock / 64) ? kGroups : ceil_div(blocks, kBlock / 64);
+#define SESSD_HELD(P, NT) hipLaunchKernelGGL((linear8_held<T, P, NT>), dim3((unsigned)groups), dim3(kBlock), 0, stream, a)
+    switch (pairs_of(a.cin)) {
+        case 1: SESSD_HELD(1, 4); break;
+        case 2: SESSD_HELD(2, 4); break;
+        case 3: case 4: SESSD_HELD(4, 4); break;
+        default: SESSD_HELD(8, 2); break;
+    }
+#undef SESSD_HELD
 }
 
 // |v| <= 448 up to a rounding of the quotient: the nearest e4m3, ties to even, as a half
@@ -117,7 +203,7 @@ uint16_t nearest_e4m3(float v) {
     return nearest_half(std::copysign(most, v), &value);
 }
 
-int padded_columns(int cout) { return ceil_div(cout, kColumns) * kColumns; }
+int padded_columns(int cin, int cout) { return ceil_div(cout, 16 * tiles_of(cin)) * 16 * tiles_of(cin); }
 
 }  // namespace
 
@@ -144,16 +230,16 @@ int Linear8Plugin::create(const sessd_linear8_desc& d, const float* weights, Lin
     for (int k = 0; k < cin; ++k)
         for (int c = 0; c < cout; ++c) p->wscale_[c] = std::fmax(p->wscale_[c], std::fabs(weights[(size_t)k * cout + c]));
     for (float& s : p->wscale_) s = std::fmax(s / 448.f, 0x1p-100f);
-    const int steps = ceil_div(cin, kStep), blocks = ceil_div(cout, kColumns);
-    std::vector<uint16_t> packed((size_t)blocks * steps * 4 * 64 * 8, 0);
+    const int tiles = tiles_of(cin), steps = 2 * pairs_of(cin), blocks = padded_columns(cin, cout) / (16 * tiles);
+    std::vector<uint16_t> packed((size_t)blocks * steps * tiles * 64 * 8, 0);
     for (int cb = 0; cb < blocks; ++cb)
-        for (int ks = 0; ks < steps; ++ks)
-            for (int t = 0; t < 4; ++t)
+        for (int s = 0; s < steps; ++s)
+            for (int t = 0; t < tiles; ++t)
                 for (int lane = 0; lane < 64; ++lane) {
-                    const int c = cb * kColumns + column_of(t, lane & 15);
-                    uint16_t* dst = packed.data() + ((((size_t)cb * steps + ks) * 4 + t) * 64 + lane) * 8;
+                    const int c = cb * 16 * tiles + column_of(tiles, t, lane & 15);
+                    uint16_t* dst = packed.data() + ((((size_t)cb * steps + s) * tiles + t) * 64 + lane) * 8;
                     for (int e = 0; e < 8; ++e) {
-                        const int k = ks * kStep + (lane >> 4) * 8 + e;
+                        const int k = channel_of(s, lane >> 4, e);
                         if (c < cout && k < cin) dst[e] = nearest_e4m3(weights[(size_t)k * cout + c] / p->wscale_[c]);
                     }
                 }
@@ -164,14 +250,13 @@ int Linear8Plugin::create(const sessd_linear8_desc& d, const float* weights, Lin
     return SESSD_OK;
 }
 
-// wscale, scale, shift for whole blocks of columns
+// factor and addend of a column, for whole blocks of columns
 int Linear8Plugin::uploadColumns() {
-    const size_t pad = (size_t)padded_columns(out_channel_);
-    std::vector<float> host(3 * pad, 0.f);
+    const size_t pad = (size_t)padded_columns(in_channel_, out_channel_);
+    std::vector<float> host(2 * pad, 0.f);
     for (int c = 0; c < out_channel_; ++c) {
-        host[c] = wscale_[c];
-        host[pad + c] = epi_.scale_host.empty() ? 1.f : epi_.scale_host[c];
-        host[2 * pad + c] = epi_.shift_host.empty() ? 0.f : epi_.shift_host[c];
+        host[c] = epi_.scale_host.empty() ? wscale_[c] : wscale_[c] * epi_.scale_host[c];
+        host[pad + c] = epi_.shift_host.empty() ? 0.f : epi_.shift_host[c];
     }
     if (!columns_dev_) SESSD_HIP_TRY(hipMalloc(reinterpret_cast<void**>(&columns_dev_), host.size() * sizeof(float)));
     SESSD_HIP_TRY(hipMemcpy(columns_dev_, host.data(), host.size() * sizeof(float), hipMemcpyHostToDevice));
@@ -254,15 +339,20 @@ int Linear8Plugin::enqueue(const sessd_tensor_desc* inputDesc, const sessd_tenso
     SESSD_TRY(check(inputDesc, outputDesc));
     if ((reinterpret_cast<uintptr_t>(inputs[0]) | reinterpret_cast<uintptr_t>(inputs[1]) | reinterpret_cast<uintptr_t>(outputs[0])) & 15)
         return fail(SESSD_E_INVALID, "linear8.enqueue: tensors must be 16-byte aligned");
-    const dim3 grid((unsigned)ceil_div(max_voxels_, kRows * (kBlock / 64)), (unsigned)ceil_div(out_channel_, kColumns));
-    const int pad = padded_columns(out_channel_), write_pad = (flags_ & SESSD_FLAG_SKIP_PAD_ROWS) ? 0 : 1;
-#define SESSD_LINEAR8(T)                                                                                                              \
-    hipLaunchKernelGGL(linear8<T>, grid, dim3(kBlock), 0, stream, static_cast<const uint8_t*>(inputs[0]),                             \
-                       static_cast<const float*>(inputs[1]), static_cast<const int32_t*>(inputs[2]), max_voxels_, in_channel_,        \
-                       out_channel_, weights_packed_dev_, columns_dev_, pad, epi_.relu, static_cast<T*>(outputs[0]), write_pad)
-    if (out_type_ == SESSD_HALF) SESSD_LINEAR8(__half);
-    else SESSD_LINEAR8(float);
-#undef SESSD_LINEAR8
+    LinearArgs a;
+    a.q = static_cast<const uint8_t*>(inputs[0]);
+    a.scale = static_cast<const float*>(inputs[1]);
+    a.voxel_num = static_cast<const int32_t*>(inputs[2]);
+    a.max_voxels = max_voxels_;
+    a.cin = in_channel_;
+    a.cout = out_channel_;
+    a.relu = epi_.relu;
+    a.write_pad = (flags_ & SESSD_FLAG_SKIP_PAD_ROWS) ? 0 : 1;
+    a.w = weights_packed_dev_;
+    a.columns = columns_dev_;
+    a.out = outputs[0];
+    if (out_type_ == SESSD_HALF) launch_linear8<__half>(a, stream);
+    else launch_linear8<float>(a, stream);
     SESSD_HIP_TRY(hipGetLastError());
     return SESSD_OK;
 }

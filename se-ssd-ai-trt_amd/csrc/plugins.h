@@ -319,7 +319,7 @@ class Linear8Plugin {
     int in_channel_ = 0, out_channel_ = 0, max_voxels_ = 0;
     std::vector<float> weights_;         // as given, FP32 [Cin][Cout]
     __half* weights_packed_dev_ = nullptr;  // e4m3 values as halves, operand order (linear8.hip)
-    float* columns_dev_ = nullptr;       // wscale, scale, shift: three rows of out_channel_ floats, padded (linear8.hip)
+    float* columns_dev_ = nullptr;       // factor and addend of each column (linear8.hip)
     Epilogue epi_;                       // (host side; the device has it in columns_dev_)
     int out_type_ = SESSD_FLOAT;
     int flags_ = 0;

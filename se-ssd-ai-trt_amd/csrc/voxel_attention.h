@@ -2,12 +2,15 @@
 //
 // A workgroup of four waves takes up to 64 queries of one window and a few heads, and walks over the window's keys in blocks of 64 (32
 // where a head's values are many).  Keys, values and voxels of a block lie in LDS; those of the next one are gathered into registers in
-// the meantime.  A wave has 16 queries; where the window has fewer than 64, waves share queries and deal the heads out.
+// the meantime.  A wave has 16 queries; where the window has fewer than 64, waves share queries and deal the heads out.  Windows of up to
+// 32 rows are a wave's own affair: their queries are their keys, which it keeps in registers, and nobody waits for anybody.
 //
 // Scores are taken transposed, S^T = K Q^T: a lane of the result has one query (its column) and four keys, so that maximum and sum over the
 // keys are mostly the lane's own, and the weights are where the second product, O^T = V^T P^T, wants them.  Maximum and sum run along
 // with the blocks; sums that are there already are rescaled only where a block raises a maximum.
 #pragma once
+
+#include <type_traits>
 
 #include "voxel_windows.h"
 
@@ -20,9 +23,11 @@ struct AttentionArgs {
     const float* slopes;  // or null
     WindowIndex w;
     int heads, kv_heads, dim;
-    float scale;          // of the scores, to the base 2 where they are not capped; 2 / cap of it, to the base 2, where they are
-    float cap;            // to the base 2; 0 = none
-    bool series;          // small capped scores by the first terms of the series: the exponential form is not exact enough
+    // A weight is 2^(by z - by max z), by > 0, z = f(q.k) - slope * to_slope * distance
+    float by, to_slope;
+    bool negate;          // the scale of the scores is negative: queries change their sign
+    bool capped, series;  // series: small scores by the first terms of the series, the exponential form is not exact enough
+    float in_cap;         // tanh(u) is taken of u = scale * q.k / cap: 2 u to the base 2 is q.k times this
     float cell_x, cell_y, cell_z;
     int write_pad;
 };
@@ -60,57 +65,73 @@ template <typename T, int DP> struct Operand;
 template <int DP> struct Operand<_Float16, DP> {
     static constexpr int kPer = 8, kPitch = DP + 8, kParts = DP >= 32 ? DP / 32 : 1;
     // 16x16x32: of row lane % 16 the eight values from 32 s + 8 (lane / 16) on; 16x16x16 where a head has 16 values: four from 4 (lane / 16)
+    typedef std::conditional_t<(DP >= 32), v8h, v4h> Part;
     struct Row {
-        v8h part[kParts];
+        Part part[kParts];
     };
-    static __device__ __forceinline__ Row query(const _Float16* p, int dim, int g) {
+    // a row's values in memory, zeros behind the last one
+    static __device__ __forceinline__ Row load(const _Float16* p, int dim, int g) {
+        constexpr int kEach = DP >= 32 ? 8 : 4;
         Row q;
 #pragma unroll
         for (int s = 0; s < kParts; ++s) {
-            v8h x = {};
-            if constexpr (DP >= 32) {
-                if (s * 32 + g * 8 < dim) x = *reinterpret_cast<const v8h*>(p + s * 32 + g * 8);
-            } else {
-                v4h y = {};
-                if (g * 4 < dim) y = *reinterpret_cast<const v4h*>(p + g * 4);
-                x = v8h{y[0], y[1], y[2], y[3], 0, 0, 0, 0};
-            }
-            q.part[s] = x;
+            q.part[s] = Part{};
+            if (s * 32 + g * kEach < dim) q.part[s] = *reinterpret_cast<const Part*>(p + s * 32 + g * kEach);
         }
         return q;
     }
-    // 16 keys from `k` on times 16 queries
+    static __device__ __forceinline__ v4f product(const Part& k, const Part& q, v4f acc) {
+        if constexpr (DP >= 32) return __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q, acc, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x16f16(k, q, acc, 0, 0, 0);
+    }
+    // 16 keys times 16 queries; keys in LDS from `k` on, or in registers
     static __device__ __forceinline__ v4f scores(const _Float16* k, const Row& q, int r, int g) {
         v4f acc = {};
 #pragma unroll
-        for (int s = 0; s < kParts; ++s) {
-            if constexpr (DP >= 32)
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const v8h*>(k + r * kPitch + s * 32 + g * 8), q.part[s], acc, 0, 0, 0);
-            else
-                acc = __builtin_amdgcn_mfma_f32_16x16x16f16(*reinterpret_cast<const v4h*>(k + r * kPitch + g * 4),
-                                                            v4h{q.part[s][0], q.part[s][1], q.part[s][2], q.part[s][3]}, acc, 0, 0, 0);
-        }
+        for (int s = 0; s < kParts; ++s) acc = product(*reinterpret_cast<const Part*>(k + r * kPitch + s * 32 + g * (DP >= 32 ? 8 : 4)), q.part[s], acc);
         return acc;
     }
-    // 32 weights of a query, rounded to 11 bits: the product's own operands are FP16
-    struct Weights {
-        v8h p;
-    };
-    static __device__ __forceinline__ Weights weights(const v4f& s, const v4f& t) {
-        Weights w;
+    static __device__ __forceinline__ v4f scores(const Row& k, const Row& q) {
+        v4f acc = {};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w.p[e] = (_Float16)s[e], w.p[4 + e] = (_Float16)t[e];
-        return w;
+        for (int s = 0; s < kParts; ++s) acc = product(k.part[s], q.part[s], acc);
+        return acc;
     }
-    // sums of 16 values from 16 b on over 32 keys: LDS transposes four keys' values as it reads them, a lane gets value lane % 16 of keys
-    // 4 (lane / 16) .. + 3 of either half, which is where its weights are
-    static __device__ __forceinline__ v4f values(const _Float16* v, const Weights& w, v4f acc, int b, int r, int g) {
+    // The weights of 16 H keys, rounded to 11 bits: the product's own operands are FP16.  Their sum is taken by a product with ones, of the
+    // weights as they are rounded.
+    template <int H> struct Weights {
+        std::conditional_t<H == 1, v4h, v8h> p[(H + 1) / 2];
+        __device__ __forceinline__ Weights(const v4f (&z)[H]) {
+#pragma unroll
+            for (int e = 0; e < 4 * H; ++e) p[e / 8][e % 8] = (_Float16)z[e / 4][e % 4];
+        }
+    };
+    typedef v4f Sum;
+    template <int H> static __device__ __forceinline__ Sum add(Sum s, const Weights<H>& w) {
+        constexpr _Float16 k1 = 1;
+        if constexpr (H == 1) return __builtin_amdgcn_mfma_f32_16x16x16f16(v4h{k1, k1, k1, k1}, w.p[0], s, 0, 0, 0);
+        else
+#pragma unroll
+            for (int t = 0; t < H / 2; ++t) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8h{k1, k1, k1, k1, k1, k1, k1, k1}, w.p[t], s, 0, 0, 0);
+        return s;
+    }
+    static __device__ __forceinline__ float sum(const Sum& s) { return s[0]; }
+    // sums of 16 values from 16 b on over 16 H keys: LDS transposes four keys' values as it reads them, a lane gets value lane % 16 of keys
+    // 4 (lane / 16) .. + 3 of each 16, which is where its weights are
+    template <int H> static __device__ __forceinline__ v4f values(const _Float16* v, const Weights<H>& w, v4f acc, int b, int r, int g) {
         typedef __attribute__((address_space(3))) v4s* lds;
         const _Float16* p = v + (4 * g + (r >> 2)) * kPitch + 16 * b + (r & 3) * 4;
-        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)p);
-        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(p + 16 * kPitch));
-        const v4h x = __builtin_bit_cast(v4h, lo), y = __builtin_bit_cast(v4h, hi);
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(v8h{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, w.p, acc, 0, 0, 0);
+        if constexpr (H == 1) {
+            return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(v4h, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)p)), w.p[0], acc, 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int t = 0; t < H / 2; ++t) {
+                const v4h x = __builtin_bit_cast(v4h, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(p + 32 * t * kPitch)));
+                const v4h y = __builtin_bit_cast(v4h, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(p + (32 * t + 16) * kPitch)));
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8h{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, w.p[t], acc, 0, 0, 0);
+            }
+            return acc;
+        }
     }
     static __device__ __forceinline__ void store(_Float16* p, v4f x) { *reinterpret_cast<v4h*>(p) = v4h{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]}; }
 };
@@ -121,33 +142,50 @@ template <int DP> struct Operand<float, DP> {
     struct Row {
         v4f part[kParts];
     };
-    static __device__ __forceinline__ Row query(const float* p, int dim, int g) {
+    static __device__ __forceinline__ Row load(const float* p, int dim, int g) {
         Row q;
 #pragma unroll
         for (int s = 0; s < kParts; ++s) {
-            v4f x = {};
-            if (s * 16 + g * 4 < dim) x = *reinterpret_cast<const v4f*>(p + s * 16 + g * 4);
-            q.part[s] = x;
+            q.part[s] = v4f{0, 0, 0, 0};
+            if (s * 16 + g * 4 < dim) q.part[s] = *reinterpret_cast<const v4f*>(p + s * 16 + g * 4);
         }
         return q;
+    }
+    static __device__ __forceinline__ v4f product(const v4f& k, const v4f& q, v4f acc) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(k[j], q[j], acc, 0, 0, 0);
+        return acc;
     }
     static __device__ __forceinline__ v4f scores(const float* k, const Row& q, int r, int g) {
         v4f acc = {};
 #pragma unroll
-        for (int s = 0; s < kParts; ++s) {
-            const v4f x = *reinterpret_cast<const v4f*>(k + r * kPitch + s * 16 + g * 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], q.part[s][j], acc, 0, 0, 0);
-        }
+        for (int s = 0; s < kParts; ++s) acc = product(*reinterpret_cast<const v4f*>(k + r * kPitch + s * 16 + g * 4), q.part[s], acc);
         return acc;
     }
-    struct Weights {
-        v4f p[2];
-    };
-    static __device__ __forceinline__ Weights weights(const v4f& s, const v4f& t) { return Weights{{s, t}}; }
-    static __device__ __forceinline__ v4f values(const float* v, const Weights& w, v4f acc, int b, int r, int g) {
+    static __device__ __forceinline__ v4f scores(const Row& k, const Row& q) {
+        v4f acc = {};
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int s = 0; s < kParts; ++s) acc = product(k.part[s], q.part[s], acc);
+        return acc;
+    }
+    template <int H> struct Weights {
+        v4f p[H];
+        __device__ __forceinline__ Weights(const v4f (&z)[H]) {
+#pragma unroll
+            for (int t = 0; t < H; ++t) p[t] = z[t];
+        }
+    };
+    typedef float Sum;
+    template <int H> static __device__ __forceinline__ Sum add(Sum s, const Weights<H>& w) {
+        float x = 0.f;
+#pragma unroll
+        for (int t = 0; t < H; ++t) x += (w.p[t][0] + w.p[t][1]) + (w.p[t][2] + w.p[t][3]);
+        return s + x;
+    }
+    static __device__ __forceinline__ float sum(const Sum& s) { return sum_of_query(s); }
+    template <int H> static __device__ __forceinline__ v4f values(const float* v, const Weights<H>& w, v4f acc, int b, int r, int g) {
+#pragma unroll
+        for (int t = 0; t < H; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 acc = __builtin_amdgcn_mfma_f32_16x16x4f32(v[(16 * t + 4 * g + e) * kPitch + 16 * b + r], w.p[t][e], acc, 0, 0, 0);
@@ -162,78 +200,286 @@ struct AttentionShape {
     using Type = T;
     using Op = Operand<T, DP>;
     static constexpr int kDim = DP, HG = HG_, KVG = KVG_, KB = KB_;
+    // 16 keys each, that a wave takes at once (two heads of 64 values: 6.1 ms at 30 000 keys with 4, 5.8 with 2, whose sums leave registers)
+    static constexpr int H = KB == 64 && HG * DP < 128 ? 4 : 2;
     static constexpr int kHalf = KVG * KB * Op::kPitch;                                  // keys, or values, in LDS
+    static constexpr int kTiny = kAttentionBlock / 64 * kTinyRows * Op::kPitch;          // the values of a tiny window for each wave
     static constexpr int kWordsHead = DP / Op::kPer;                                     // 16-byte words of a head's row
     static constexpr int kLoads = (2 * KVG * kWordsHead * KB + kAttentionBlock - 1) / kAttentionBlock;  // of a thread
 };
 
 enum { kCapNone, kCapExponential, kCapSeries };
 
-// 16 H keys times 16 queries of a head: scores, running maximum and sum, weights, products with the values
-template <typename S, int CAP, bool BIAS, int H>
-__device__ __forceinline__ void attend_block(const AttentionArgs& a, const typename S::Type* k, const typename S::Type* v, const typename S::Op::Row& q,
-                                             const float (&far)[S::KB / 16][4], float slope, int left, float& most, float& total,
-                                             v4f (&acc)[S::kDim / 16], int r, int g) {
+constexpr int kEnoughGroups = 1024;  // workgroups: four waves on every SIMD of 256 compute units
+
+// 16 H keys and 16 queries of a head: from z = q.k on to the weights, running maximum and sum, products with the values at `v`
+template <typename S, int CAP, bool BIAS, int H, bool TAIL>
+__device__ __forceinline__ void attend(const AttentionArgs& a, v4f (&z)[H], const typename S::Type* v, const float (&far)[H][4], float slope,
+                                       int left, float& most, typename S::Op::Sum& total, v4f (&acc)[S::kDim / 16], int r, int g) {
     using Op = typename S::Op;
-    v4f s[H];
 #pragma unroll
-    for (int t = 0; t < H; ++t) {
-        s[t] = Op::scores(k + 16 * t * Op::kPitch, q, r, g);
+    for (int t = 0; t < H; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float x = s[t][e] * a.scale;
+            float x = z[t][e];
             if constexpr (CAP != kCapNone) {
-                // cap * tanh(u) = cap - 2 cap / (1 + e^2u); near 0, where that has lost the last bits relative to u, the first terms of the
-                // series (the next one is below 2^-24 of the sum for |u| < 0.2)
-                const float y = fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x)), a.cap);
+                // tanh(u) = 1 - 2 / (1 + e^2u), of which the exponential form's z is the half that depends on u; near 0, where that has lost
+                // the last bits relative to u, the first terms of the series (the next one is below 2^-24 of the sum for |u| < 0.2)
+                const float y = x * a.in_cap, f = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(y));
                 if constexpr (CAP == kCapSeries) {
-                    const float u = x * (0.5f / kLog2e), u2 = u * u;
-                    const float near = a.cap * u * (1.f + u2 * (-1.f / 3.f + u2 * (2.f / 15.f + u2 * (-17.f / 315.f))));
-                    x = fabsf(u) < 0.2f ? near : y;
+                    const float u = y * (0.5f / kLog2e), u2 = u * u;
+                    const float near = u * (1.f + u2 * (-1.f / 3.f + u2 * (2.f / 15.f + u2 * (-17.f / 315.f))));
+                    x = fabsf(u) < 0.2f ? near : fmaf(-2.f, f, 1.f);
                 } else {
-                    x = y;
+                    x = -f;
                 }
             }
             if constexpr (BIAS) x = fmaf(-slope, far[t][e], x);
-            s[t][e] = x;
+            z[t][e] = x;
         }
-    }
-    if (left < 16 * H) {
+    if constexpr (TAIL) {  // (keys that there are not)
 #pragma unroll
         for (int t = 0; t < H; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[t][e] = 16 * t + 4 * g + e < left ? s[t][e] : -INFINITY;
+            for (int e = 0; e < 4; ++e) z[t][e] = 16 * t + 4 * g + e < left ? z[t][e] : -INFINITY;
     }
     float block_most = -INFINITY;
 #pragma unroll
     for (int t = 0; t < H; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) block_most = fmaxf(block_most, s[t][e]);
+        for (int e = 0; e < 4; ++e) block_most = fmaxf(block_most, z[t][e]);
     if (__any(block_most > most)) {
         const float new_most = fmaxf(most, most_of_query(block_most));
-        const float shrink = most == new_most ? 1.f : __builtin_amdgcn_exp2f(most - new_most);
+        const float shrink = most == new_most ? 1.f : __builtin_amdgcn_exp2f((most - new_most) * a.by);
         most = new_most;
         total *= shrink;
 #pragma unroll
         for (int b = 0; b < S::kDim / 16; ++b) acc[b] *= shrink;
     }
     // (scores of -infinity alone leave nothing to subtract: they weigh 0, and 0 / 0 at the end)
-    const float less = most == -INFINITY ? 0.f : most;
-    float sum[H];
+    const float less = most == -INFINITY ? 0.f : most * a.by;
+#pragma unroll
+    for (int t = 0; t < H; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[t][e] = __builtin_amdgcn_exp2f(fmaf(z[t][e], a.by, -less));
+    const typename Op::template Weights<H> p(z);
+    total = Op::template add<H>(total, p);
+#pragma unroll
+    for (int b = 0; b < S::kDim / 16; ++b) acc[b] = Op::template values<H>(v, p, acc[b], b, r, g);
+}
+
+// A voxel's place in its window, in the unit of the slopes
+__device__ __forceinline__ float4 place_of(const AttentionArgs& a, const float4& c) { return make_float4(c.x * a.cell_x, c.y * a.cell_y, c.z * a.cell_z, 0.f); }
+__device__ __forceinline__ float distance(const float4& c, const float4& d) {
+    const float dx = c.x - d.x, dy = c.y - d.y, dz = c.z - d.z;
+    return __builtin_amdgcn_sqrtf(fmaf(dx, dx, fmaf(dy, dy, dz * dz)));
+}
+
+template <typename S>
+__device__ __forceinline__ void store_row(const AttentionArgs& a, int row, int head, const typename S::Op::Sum& total, const v4f (&acc)[S::kDim / 16],
+                                          bool there, int g) {
+    using Op = typename S::Op;
+    const float by = 1.f / Op::sum(total);
+    typename S::Type* dst = static_cast<typename S::Type*>(a.out) + ((size_t)(unsigned)row * a.heads + head) * a.dim;
+#pragma unroll
+    for (int b = 0; b < S::kDim / 16; ++b)
+        if (there && 16 * b + 4 * g < a.dim) Op::store(dst + 16 * b + 4 * g, acc[b] * by);
+}
+
+template <typename S>
+__device__ __forceinline__ typename S::Op::Row load_query(const AttentionArgs& a, const typename S::Type* row, int head, int g) {
+    typename S::Op::Row q = S::Op::load(row + head * a.dim, a.dim, g);
+    if (a.negate)
+#pragma unroll
+        for (int s = 0; s < S::Op::kParts; ++s) q.part[s] = -q.part[s];
+    return q;
+}
+
+// A window of up to 16 H rows and a head, by one wave
+template <typename S, int CAP, bool BIAS, int H>
+__device__ __forceinline__ void tiny_window(const AttentionArgs& a, int start, int len, int head, typename S::Type* s_v) {
+    using T = typename S::Type;
+    using Op = typename S::Op;
+    constexpr int kWords = 16 * H * S::kWordsHead, kLoads = (kWords + 63) / 64;  // words of the values, of a lane
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int kv = head / (a.heads / a.kv_heads);
+    const size_t stride = (size_t)(a.heads + 2 * a.kv_heads) * a.dim;
+    const T* const qkv = static_cast<const T*>(a.qkv);
+    const auto place = [&](int i) { return start + (i < len ? i : len - 1); };
+    int row[H];
+    v4u word[kLoads];
+    typename Op::Row q[H], k[H];
+    float4 me[H], them[H][4];
 #pragma unroll
     for (int t = 0; t < H; ++t) {
+        row[t] = a.w.order[place(16 * t + r)];
+        if constexpr (BIAS) {
+            me[t] = a.w.cell[place(16 * t + r)];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[t][e] = __builtin_amdgcn_exp2f(s[t][e] - less);
-        sum[t] = (s[t][0] + s[t][1]) + (s[t][2] + s[t][3]);
+            for (int e = 0; e < 4; ++e) them[t][e] = a.w.cell[place(16 * t + 4 * g + e)];
+        }
+    }
+    int value_row[kLoads];
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) value_row[j] = a.w.order[place((64 * j + lane) / S::kWordsHead)];
+#pragma unroll
+    for (int t = 0; t < H; ++t) {
+        q[t] = load_query<S>(a, qkv + (size_t)(unsigned)row[t] * stride, head, g);
+        k[t] = Op::load(qkv + (size_t)(unsigned)row[t] * stride + (size_t)(a.heads + kv) * a.dim, a.dim, g);
     }
 #pragma unroll
-    for (int t = 0; t < H; t += 2) total += sum[t] + sum[t + 1];
-#pragma unroll
-    for (int t = 0; t < H; t += 2) {
-        const typename Op::Weights p = Op::weights(s[t], s[t + 1]);
-#pragma unroll
-        for (int b = 0; b < S::kDim / 16; ++b) acc[b] = Op::values(v + 16 * t * Op::kPitch, p, acc[b], b, r, g);
+    for (int j = 0; j < kLoads; ++j) {
+        const int key = (64 * j + lane) / S::kWordsHead, d = (64 * j + lane) % S::kWordsHead * Op::kPer;
+        word[j] = v4u{0, 0, 0, 0};
+        if (key < len && d < a.dim)
+            word[j] = *reinterpret_cast<const v4u*>(qkv + (size_t)(unsigned)value_row[j] * stride + (size_t)(a.heads + a.kv_heads + kv) * a.dim + d);
     }
+    const float slope = BIAS ? a.slopes[head] * a.to_slope : 0.f;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+        const int key = (64 * j + lane) / S::kWordsHead, d = (64 * j + lane) % S::kWordsHead * Op::kPer;
+        if (key < 16 * H) *reinterpret_cast<v4u*>(s_v + key * Op::kPitch + d) = word[j];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int u = 0; u < H; ++u) {  // 16 queries
+        float far[H][4];
+        v4f z[H];
+#pragma unroll
+        for (int t = 0; t < H; ++t) {
+            z[t] = Op::scores(k[t], q[u]);
+            if constexpr (BIAS) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) far[t][e] = distance(place_of(a, them[t][e]), place_of(a, me[u]));
+            }
+        }
+        float most = -INFINITY;
+        typename Op::Sum total = {};
+        v4f acc[S::kDim / 16] = {};
+        attend<S, CAP, BIAS, H, true>(a, z, s_v, far, slope, len, most, total, acc, r, g);
+        store_row<S>(a, row[u], head, total, acc, 16 * u + r < len, g);
+    }
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Up to 64 queries of a window from q0 on and heads h_first .. h_first + hc - 1, by the workgroup
+template <typename S, int CAP, bool BIAS>
+__device__ __forceinline__ void window_rows(const AttentionArgs& a, int start, int len, int q0, int h_first, int hc, typename S::Type* s_kv, float4* s_cell,
+                                            int32_t* s_row) {
+    using T = typename S::Type;
+    using Op = typename S::Op;
+    constexpr int HG = S::HG, KB = S::KB, kLoads = S::kLoads;
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const T* const qkv = static_cast<const T*>(a.qkv);
+    const int ratio = a.heads / a.kv_heads;
+    const int kv_first = h_first / ratio, kvs = (h_first + hc - 1) / ratio - kv_first + 1;
+    const unsigned stride = (unsigned)(a.heads + 2 * a.kv_heads) * (unsigned)a.dim;
+
+    const int32_t* const order = a.w.order + start;
+    const float4* const cells = a.w.cell + start;
+
+    // Words of a block: key by key, of each the key's heads and then the value's, rounded up to a power of two.  A thread has words tid,
+    // tid + 256, ...: the same ones of every step-th key.
+    const int kv_words = (kvs > 2 ? 4 : kvs) * S::kWordsHead, step = kAttentionBlock / (2 * kv_words);
+    const int word_at = tid & (2 * kv_words - 1), word_half = word_at >= kv_words ? 1 : 0, word_head = (word_at & (kv_words - 1)) / S::kWordsHead;
+    const int word_d = word_at % S::kWordsHead * Op::kPer;
+    const bool word_there = word_head < kvs && tid / (2 * kv_words) < KB;
+    const int first_key = word_there && word_d < a.dim ? tid / (2 * kv_words) : 0x40000000;  // (beyond every key: no word)
+    const T* const source = qkv + (size_t)(a.heads + kv_first + word_half * a.kv_heads + word_head) * a.dim + word_d;
+    T* const target = s_kv + word_half * S::kHalf + (word_head * KB + tid / (2 * kv_words)) * Op::kPitch + word_d;
+
+    const int tiles = len - q0 >= kItemRows ? 4 : (len - q0 + 15) / 16;
+    // waves of a tile of 16 queries, and this wave's heads
+    const int share = tiles == 1 ? 4 : tiles == 2 ? 2 : 1;
+    const int per = (hc + share - 1) / share;
+    const int tile = wave / share, h0 = wave % share * per;
+    const int mine = tile >= tiles || h0 >= hc ? 0 : hc - h0 < per ? hc - h0 : per;
+
+    v4u word[kLoads];  // (a thread's words of the next block: those of keys that there are)
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+        if (i * step < KB && first_key + i * step < len) word[i] = *reinterpret_cast<const v4u*>(source + (size_t)(unsigned)order[first_key + i * step] * stride);
+    float4 cell = make_float4(0, 0, 0, 0);
+    int32_t row = 0;
+    if (tid < KB) {
+        if (BIAS) cell = cells[tid < len ? tid : 0];
+        row = order[KB + tid < len ? KB + tid : 0];
+    }
+    const int q_at = q0 + tile * 16 + r;
+    const bool q_there = q_at < len && mine > 0;
+    const int q_row = order[q_there ? q_at : 0];
+    float4 me = make_float4(0, 0, 0, 0);
+    if (BIAS) me = place_of(a, cells[q_there ? q_at : 0]);
+    typename Op::Row q[HG];
+    float slope[HG], most[HG];
+    typename Op::Sum total[HG];
+    v4f acc[HG][S::kDim / 16];
+#pragma unroll
+    for (int i = 0; i < HG; ++i) {
+        const int head = h_first + (i < mine ? h0 + i : 0);
+        q[i] = load_query<S>(a, qkv + (size_t)(unsigned)q_row * stride, head, g);
+        slope[i] = BIAS ? a.slopes[head] * a.to_slope : 0.f;
+        most[i] = -INFINITY;
+        total[i] = typename Op::Sum{};
+#pragma unroll
+        for (int b = 0; b < S::kDim / 16; ++b) acc[i][b] = v4f{0, 0, 0, 0};
+    }
+    for (int k0 = 0; k0 < len; k0 += KB) {
+        const int left = len - k0;
+        __syncthreads();  // (the block before, or the item before, is worked on)
+        if (k0 == 0 && word_there && word_d >= a.dim)  // values behind a head's last one are zeros
+            for (int key = 0; tid / (2 * kv_words) + key < KB; key += step) *reinterpret_cast<v4u*>(target + key * Op::kPitch) = v4u{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+            if (first_key + i * step < KB) *reinterpret_cast<v4u*>(target + i * step * Op::kPitch) = first_key + i * step < left ? word[i] : v4u{0, 0, 0, 0};
+        if (tid < KB) {
+            if (BIAS) s_cell[tid] = place_of(a, cell);
+            s_row[tid] = row;
+        }
+        __syncthreads();
+        if (left > KB) {  // the next block, and the rows of the one behind it
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i)
+                if (i * step < KB && first_key + i * step < left - KB)
+                    word[i] = *reinterpret_cast<const v4u*>(source + (size_t)(unsigned)s_row[first_key + i * step] * stride);
+            if (tid < KB) {
+                if (BIAS) cell = cells[KB + tid < left ? k0 + KB + tid : 0];
+                row = order[2 * KB + tid < left ? k0 + 2 * KB + tid : 0];
+            }
+        }
+        if (mine > 0) {
+            const auto keys = [&](auto sixteens, auto tail, int k1) {  // 16 H keys from k1 on
+                constexpr int H = decltype(sixteens)::value;
+                constexpr bool TAIL = decltype(tail)::value;
+                float far[H][4];
+                if constexpr (BIAS) {
+#pragma unroll
+                    for (int t = 0; t < H; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) far[t][e] = distance(s_cell[k1 + 16 * t + 4 * g + e], me);
+                }
+#pragma unroll
+                for (int i = 0; i < HG; ++i) {
+                    if (i >= mine) continue;
+                    const T* k = s_kv + (((h_first + h0 + i) / ratio - kv_first) * KB + k1) * Op::kPitch;
+                    v4f z[H];
+#pragma unroll
+                    for (int t = 0; t < H; ++t) z[t] = Op::scores(k + 16 * t * Op::kPitch, q[i], r, g);
+                    attend<S, CAP, BIAS, H, TAIL>(a, z, k + S::kHalf, far, slope[i], left - k1, most[i], total[i], acc[i], r, g);
+                }
+            };
+            int k1 = 0;
+#pragma unroll 1
+            for (; k1 < KB && k1 + 16 * S::H <= left; k1 += 16 * S::H) keys(std::integral_constant<int, S::H>{}, std::false_type{}, k1);
+#pragma unroll 1
+            for (; k1 < KB && k1 < left; k1 += 32) keys(std::integral_constant<int, 2>{}, std::true_type{}, k1);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < HG; ++i)
+        if (i < mine) store_row<S>(a, q_row, h_first + h0 + i, total[i], acc[i], q_there, g);
 }
 
 template <typename S, int CAP, bool BIAS>
@@ -241,148 +487,108 @@ __global__ void __launch_bounds__(kAttentionBlock, 2)
 voxel_attention(AttentionArgs a) {
     using T = typename S::Type;
     using Op = typename S::Op;
-    constexpr int HG = S::HG, KB = S::KB, kBlocks = S::kDim / 16, kLoads = S::kLoads;
-    __shared__ __align__(16) T s_kv[2 * S::kHalf];  // [keys, values][kv head][key][kPitch]
-    __shared__ float4 s_cell[KB];
-    __shared__ int32_t s_row[KB];                   // rows of the block to come
-    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const T* const qkv = static_cast<const T*>(a.qkv);
+    __shared__ __align__(16) T s_kv[2 * S::kHalf > S::kTiny ? 2 * S::kHalf : S::kTiny];  // [keys, values][kv head][key][kPitch]; tiny windows: [wave][key][kPitch]
+    __shared__ float4 s_cell[S::KB];
+    __shared__ int32_t s_row[S::KB];                // rows of the block to come
     T* const out = static_cast<T*>(a.out);
-    const int h_first = blockIdx.y * HG;
-    const int hc = a.heads - h_first < HG ? a.heads - h_first : HG;  // heads of this workgroup
-    const int ratio = a.heads / a.kv_heads;
-    const int kv_first = h_first / ratio, kvs = (h_first + hc - 1) / ratio - kv_first + 1;
-    const unsigned stride = (unsigned)(a.heads + 2 * a.kv_heads) * (unsigned)a.dim;
-    const T* const keys = qkv + (size_t)(a.heads + kv_first) * a.dim;
-
-    // Words of a block: key by key, of each the key's heads and then the value's.  A thread has words tid, tid + 256, ...
-    const int words_key = 2 * kvs * S::kWordsHead;
-    int key_of[kLoads], from[kLoads], to[kLoads];
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-        const int c = i * kAttentionBlock + tid;
-        const int key = c / words_key, rest = c - key * words_key;
-        const int half = rest >= words_key / 2 ? 1 : 0, at = rest - half * (words_key / 2);
-        const int head = at / S::kWordsHead, d = at % S::kWordsHead * Op::kPer;
-        key_of[i] = key < KB && d < a.dim ? key : 0x40000000;
-        from[i] = half * a.kv_heads * a.dim + head * a.dim + d;
-        to[i] = half * S::kHalf + (head * KB + key) * Op::kPitch + d;
-        // (values behind a head's last one are zeros, here and for good)
-        if (key < KB && d >= a.dim) *reinterpret_cast<v4u*>(s_kv + to[i]) = v4u{0, 0, 0, 0};
-    }
-
-    const int longs = a.w.head[kHeadLong], items = longs + a.w.head[kHeadShort];
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
-        const int4 it = window_item(a.w, item, longs);
-        const int start = __builtin_amdgcn_readfirstlane(it.x), len = __builtin_amdgcn_readfirstlane(it.y), q0 = __builtin_amdgcn_readfirstlane(it.z);
-        const int32_t* const order = a.w.order + start;
-        const float4* const cells = a.w.cell + start;
-        const int tiles = len - q0 >= kItemRows ? 4 : (len - q0 + 15) / 16;
-        // waves of a tile of 16 queries, and this wave's heads
-        const int share = tiles == 1 ? 4 : tiles == 2 ? 2 : 1;
-        const int per = (HG + share - 1) / share;
-        const int tile = wave / share, h0 = wave % share * per;
-        const int mine = tile >= tiles || h0 >= hc ? 0 : hc - h0 < per ? hc - h0 : per;
-
-        v4u word[kLoads];  // (a thread's words of the next block: those of keys that there are)
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-            if (key_of[i] < len) word[i] = *reinterpret_cast<const v4u*>(keys + (size_t)(unsigned)order[key_of[i]] * stride + from[i]);
-        float4 cell = make_float4(0, 0, 0, 0);
-        int32_t row = 0;
-        if (tid < KB) {
-            if (BIAS) cell = cells[tid < len ? tid : 0];
-            row = order[KB + tid < len ? KB + tid : 0];
-        }
-        const int q_at = q0 + tile * 16 + r;
-        const bool q_there = q_at < len && mine > 0;
-        const int q_row = order[q_there ? q_at : 0];
-        float4 me = make_float4(0, 0, 0, 0);
-        if (BIAS) me = cells[q_there ? q_at : 0];
-        typename Op::Row q[HG];
-        float slope[HG], most[HG], total[HG];
-        v4f acc[HG][kBlocks];
-#pragma unroll
-        for (int i = 0; i < HG; ++i) {
-            const int head = h_first + (i < mine ? h0 + i : 0);
-            q[i] = Op::query(qkv + (size_t)(unsigned)q_row * stride + head * a.dim, a.dim, g);
-            slope[i] = BIAS ? a.slopes[head] * kLog2e : 0.f;
-            most[i] = -INFINITY;
-            total[i] = 0.f;
-#pragma unroll
-            for (int b = 0; b < kBlocks; ++b) acc[i][b] = v4f{0, 0, 0, 0};
-        }
-        for (int k0 = 0; k0 < len; k0 += KB) {
-            const int left = len - k0;
-            __syncthreads();  // (the block before, or the item before, is worked on)
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i)
-                if (key_of[i] < KB) *reinterpret_cast<v4u*>(s_kv + to[i]) = key_of[i] < left ? word[i] : v4u{0, 0, 0, 0};
-            if (tid < KB) {
-                if (BIAS) s_cell[tid] = cell;
-                s_row[tid] = row;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int longs = a.w.head[kHeadLong], shorts = a.w.head[kHeadShort], tinies = a.w.head[kHeadTiny];
+    // Heads of a workgroup: all that it can take where that leaves workgroups enough, else one.  (Groups of heads of an item side by side: long
+    // items come first, and share what L2 has of the rows.)
+    const int all = (a.heads + S::HG - 1) / S::HG;
+    const int per_long = longs * all >= kEnoughGroups ? S::HG : 1, per_short = (longs + shorts) * all >= kEnoughGroups ? S::HG : 1;
+    const int groups_long = (a.heads + per_long - 1) / per_long, groups_short = (a.heads + per_short - 1) / per_short;
+    const int end_long = longs * groups_long, end_short = end_long + shorts * groups_short, end = end_short + (tinies + 3) / 4 * a.heads;
+    for (int v = blockIdx.x; v < end; v += gridDim.x) {
+        if (v < end_short) {
+            const bool is_long = v < end_long;
+            const int u = is_long ? v : v - end_long, gs = is_long ? groups_long : groups_short, per = is_long ? per_long : per_short;
+            const int4 it = is_long ? long_item(a.w, u / gs) : short_item(a.w, u / gs);
+            const int h = u % gs * per;
+            const int start = __builtin_amdgcn_readfirstlane(it.x);
+            window_rows<S, CAP, BIAS>(a, start, __builtin_amdgcn_readfirstlane(it.y), __builtin_amdgcn_readfirstlane(it.z), h,
+                                      a.heads - h < per ? a.heads - h : per, s_kv, s_cell, s_row);
+        } else {
+            // (the heads of a window side by side)
+            const int u = v - end_short, at = u / a.heads * 4 + wave, h = u % a.heads;
+            __syncthreads();  // (an item of the other kind is worked on)
+            if (at < tinies) {
+                const int2 it = a.w.tiny[at];
+                const int start = __builtin_amdgcn_readfirstlane(it.x), len = __builtin_amdgcn_readfirstlane(it.y);
+                T* const s_v = s_kv + wave * kTinyRows * Op::kPitch;
+                if (len <= 16) tiny_window<S, CAP, BIAS, 1>(a, start, len, h, s_v);
+                else tiny_window<S, CAP, BIAS, 2>(a, start, len, h, s_v);
             }
-            __syncthreads();
-            if (left > KB) {  // the next block, and the rows of the one behind it
-#pragma unroll
-                for (int i = 0; i < kLoads; ++i)
-                    if (key_of[i] < left - KB) word[i] = *reinterpret_cast<const v4u*>(keys + (size_t)(unsigned)s_row[key_of[i]] * stride + from[i]);
-                if (tid < KB) {
-                    if (BIAS) cell = cells[KB + tid < left ? k0 + KB + tid : 0];
-                    row = order[2 * KB + tid < left ? k0 + 2 * KB + tid : 0];
-                }
-            }
-            if (mine > 0) {
-                float far[KB / 16][4];
-                if constexpr (BIAS) {
-#pragma unroll
-                    for (int t = 0; t < KB / 16; ++t)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float4 c = s_cell[16 * t + 4 * g + e];
-                            const float dx = (c.x - me.x) * a.cell_x, dy = (c.y - me.y) * a.cell_y, dz = (c.z - me.z) * a.cell_z;
-                            far[t][e] = __builtin_amdgcn_sqrtf(dx * dx + dy * dy + dz * dz);
-                        }
-                }
-#pragma unroll
-                for (int i = 0; i < HG; ++i) {
-                    if (i >= mine) continue;
-                    const T* k = s_kv + ((h_first + h0 + i) / ratio - kv_first) * KB * Op::kPitch;
-                    const T* v = k + S::kHalf;
-                    if (KB == 32 || left <= 32) attend_block<S, CAP, BIAS, 2>(a, k, v, q[i], far, slope[i], left, most[i], total[i], acc[i], r, g);
-                    else attend_block<S, CAP, BIAS, KB / 16>(a, k, v, q[i], far, slope[i], left, most[i], total[i], acc[i], r, g);
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < HG; ++i) {
-            if (i >= mine) continue;
-            const float by = 1.f / sum_of_query(total[i]);
-            T* dst = out + ((size_t)(unsigned)q_row * a.heads + h_first + h0 + i) * a.dim;
-#pragma unroll
-            for (int b = 0; b < kBlocks; ++b)
-                if (q_there && 16 * b + 4 * g < a.dim) Op::store(dst + 16 * b + 4 * g, acc[i][b] * by);
         }
     }
     // rows that attend to nothing: outside the grid, and behind the last one
     const int n = clamp_rows(a.voxel_num, a.w.max_voxels), places = a.w.head[kHeadPlaces];
     const size_t row_words = (size_t)a.heads * a.dim / Op::kPer;
-    const size_t thread = ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * kAttentionBlock + tid, threads = (size_t)gridDim.x * gridDim.y * kAttentionBlock;
+    const size_t thread = (size_t)blockIdx.x * kAttentionBlock + tid, threads = (size_t)gridDim.x * kAttentionBlock;
     for (size_t i = thread; i < (size_t)(n - places) * row_words; i += threads)
         reinterpret_cast<v4u*>(out)[(size_t)a.w.order[places + i / row_words] * row_words + i % row_words] = v4u{0, 0, 0, 0};
     if (a.write_pad)
         for (size_t i = (size_t)n * row_words + thread; i < (size_t)a.w.max_voxels * row_words; i += threads) reinterpret_cast<v4u*>(out)[i] = v4u{0, 0, 0, 0};
 }
 
+// The same where the list has spans (few rows): kFewPlaces places and a head are a workgroup's, which takes the tiny windows that begin
+// among them and the blocks of 64 queries that do.
+constexpr int kFewPlaces = 32;
+template <typename S, int CAP, bool BIAS>
+__global__ void __launch_bounds__(kAttentionBlock, 2)
+voxel_attention_few(AttentionArgs a) {
+    using T = typename S::Type;
+    using Op = typename S::Op;
+    __shared__ __align__(16) T s_kv[2 * S::kHalf > S::kTiny ? 2 * S::kHalf : S::kTiny];
+    __shared__ float4 s_cell[S::KB];
+    __shared__ int32_t s_row[S::KB];
+    T* const out = static_cast<T*>(a.out);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int first = (int)(blockIdx.x / (unsigned)a.heads) * kFewPlaces, head = (int)(blockIdx.x % (unsigned)a.heads);
+    const int n = clamp_rows(a.voxel_num, a.w.max_voxels), places = a.w.head[kHeadPlaces];
+    const int place = first + lane;
+    const bool there = lane < kFewPlaces && place < places;
+    const int2 span = there ? a.w.span[place] : make_int2(0, 0);  // (every wave has all of them)
+    const int before = place - span.x;
+    for (uint64_t m = __ballot(there && span.y > kTinyRows && before % kItemRows == 0); m; m &= m - 1) {
+        const int who = __builtin_ctzll(m);
+        window_rows<S, CAP, BIAS>(a, __builtin_amdgcn_readlane(span.x, who), __builtin_amdgcn_readlane(span.y, who), __builtin_amdgcn_readlane(before, who), head, 1,
+                                  s_kv, s_cell, s_row);
+    }
+    __syncthreads();  // (the last item is worked on)
+    int turn = 0;
+    for (uint64_t m = __ballot(there && span.y <= kTinyRows && before == 0); m; m &= m - 1, ++turn) {
+        if ((turn & 3) != wave) continue;
+        const int who = __builtin_ctzll(m), start = __builtin_amdgcn_readlane(span.x, who), len = __builtin_amdgcn_readlane(span.y, who);
+        T* const s_v = s_kv + wave * kTinyRows * Op::kPitch;
+        if (len <= 16) tiny_window<S, CAP, BIAS, 1>(a, start, len, head, s_v);
+        else tiny_window<S, CAP, BIAS, 2>(a, start, len, head, s_v);
+    }
+    // rows that attend to nothing: outside the grid, and behind the last one
+    const int words = a.dim / Op::kPer;
+    for (int i = tid; i < kFewPlaces * words; i += kAttentionBlock) {
+        const int p = first + i / words;
+        if (p < places || p >= a.w.max_voxels || (p >= n && !a.write_pad)) continue;
+        *reinterpret_cast<v4u*>(out + ((size_t)(p < n ? a.w.order[p] : p) * a.heads + head) * a.dim + i % words * Op::kPer) = v4u{0, 0, 0, 0};
+    }
+}
+
 template <typename S, int CAP, bool BIAS>
 void launch_attention_as(const AttentionArgs& a, hipStream_t stream) {
-    const dim3 grid((unsigned)(a.w.items_cap < 4096 ? a.w.items_cap : 4096), (unsigned)ceil_div(a.heads, S::HG));
-    hipLaunchKernelGGL((voxel_attention<S, CAP, BIAS>), grid, dim3(kAttentionBlock), 0, stream, a);
+    if (a.w.max_voxels <= kFewRows) {
+        using F = AttentionShape<typename S::Type, S::kDim, 1, 1, S::KB>;
+        hipLaunchKernelGGL((voxel_attention_few<F, CAP, BIAS>), dim3((unsigned)(ceil_div(a.w.max_voxels, kFewPlaces) * a.heads)), dim3(kAttentionBlock), 0, stream, a);
+        return;
+    }
+    // (a tiny window's share of a workgroup is a quarter; what is beyond the grid is taken in turns)
+    const int64_t most = ((int64_t)a.w.items_cap + ceil_div(a.w.max_voxels, 4)) * a.heads;
+    const unsigned grid = (unsigned)(most < 4096 ? most : 4096);
+    hipLaunchKernelGGL((voxel_attention<S, CAP, BIAS>), dim3(grid), dim3(kAttentionBlock), 0, stream, a);
 }
 template <typename S>
 void launch_attention_shape(const AttentionArgs& a, hipStream_t stream) {
     constexpr bool kHalf = sizeof(typename S::Type) == 2;
-    if (a.cap == 0.f) {
+    if (!a.capped) {
         if (a.slopes) launch_attention_as<S, kCapNone, true>(a, stream);
         else launch_attention_as<S, kCapNone, false>(a, stream);
     } else if (a.series) {
@@ -403,12 +609,19 @@ inline int kv_heads_of(const AttentionArgs& a, int group) {
     }
     return most;
 }
-// What a thread keeps of the next block are eight words at most: wide heads share a workgroup where they share keys.
-template <typename T, int DP, int KVG, int KB>
+// What a thread keeps of the next block are eight words at most.
+template <typename T, int DP, int KB>
 void launch_attention_dim(const AttentionArgs& a, hipStream_t stream) {
-    if constexpr (KVG == 4) launch_attention_shape<AttentionShape<T, DP, 4, 4, KB>>(a, stream);
-    else if (kv_heads_of(a, 2 * KVG) <= KVG) launch_attention_shape<AttentionShape<T, DP, 2 * KVG, KVG, KB>>(a, stream);
-    else launch_attention_shape<AttentionShape<T, DP, KVG, KVG, KB>>(a, stream);
+    // A second head uses the distances of the first; a wave's registers leave the card fewer waves.  FP16, HG 1 and 2: 16 000 voxels times 8
+    // heads of 16 values 40.5 and 43 us, 53 000 times 8 of 32 131 and 110, 30 000 times 8 of 64 in one window 5.7 and 5.8 ms (with cap).  FP32
+    // waits for the matrix cores: 61 and 77 us.
+    if constexpr (sizeof(T) == 2) {
+        if ((int64_t)a.w.max_voxels * a.heads >= 200000) {
+            if (kv_heads_of(a, 2) == 1) return launch_attention_shape<AttentionShape<T, DP, 2, 1, KB>>(a, stream);
+            if constexpr (DP <= 64) return launch_attention_shape<AttentionShape<T, DP, 2, 2, KB>>(a, stream);
+        }
+    }
+    launch_attention_shape<AttentionShape<T, DP, 1, 1, KB>>(a, stream);
 }
 
 #endif

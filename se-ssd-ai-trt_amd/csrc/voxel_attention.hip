@@ -11,10 +11,10 @@
 namespace sessd {
 
 int launch_attention_half(const AttentionArgs& a, hipStream_t stream) {
-    if (a.dim <= 16) launch_attention_dim<_Float16, 16, 4, 64>(a, stream);
-    else if (a.dim <= 32) launch_attention_dim<_Float16, 32, 4, 64>(a, stream);
-    else if (a.dim <= 64) launch_attention_dim<_Float16, 64, 2, 64>(a, stream);
-    else launch_attention_dim<_Float16, 128, 1, 64>(a, stream);
+    if (a.dim <= 16) launch_attention_dim<_Float16, 16, 64>(a, stream);
+    else if (a.dim <= 32) launch_attention_dim<_Float16, 32, 64>(a, stream);
+    else if (a.dim <= 64) launch_attention_dim<_Float16, 64, 64>(a, stream);
+    else launch_attention_dim<_Float16, 128, 64>(a, stream);
     SESSD_HIP_TRY(hipGetLastError());
     return SESSD_OK;
 }
@@ -27,6 +27,7 @@ WindowGrid grid_of(const sessd_voxelattn_desc& d) {
         g.shape[2 - a] = d.spatial_shape[a];
         g.window[2 - a] = d.window_shape[a];
         g.shift[2 - a] = d.window_shift[a];
+        g.over[2 - a] = d.window_shape[a] == 1 ? 0 : ~(uint64_t)0 / (uint64_t)d.window_shape[a] + 1;
         g.count[2 - a] = (int)(((int64_t)d.spatial_shape[a] - 1 + d.window_shift[a]) / d.window_shape[a]) + 1;
     }
     return g;
@@ -139,12 +140,17 @@ int VoxelAttentionPlugin::attend(const void* const* inputs, void* const* outputs
     a.heads = desc_.num_heads;
     a.kv_heads = desc_.num_kv_heads;
     a.dim = desc_.head_dim;
-    const double scale = desc_.softmax_scale != 0.f ? desc_.softmax_scale : 1.0 / std::sqrt((double)desc_.head_dim), log2e = 1.4426950408889634;
-    a.scale = (float)(desc_.score_cap > 0.f ? scale * log2e * 2.0 / desc_.score_cap : scale * log2e);
-    a.cap = (float)(desc_.score_cap * log2e);
+    const double scale = desc_.softmax_scale != 0.f ? std::fabs((double)desc_.softmax_scale) : 1.0 / std::sqrt((double)desc_.head_dim);
+    const double log2e = 1.4426950408889634, cap = desc_.score_cap;
+    a.negate = desc_.softmax_scale < 0.f;
+    a.capped = cap > 0.0;
     // The exponential form is within 2^-23 of the cap: of a score's own size in FP32 from caps of some hundreds on, below FP16's rounding of
     // the weights up to 512.
-    a.series = !half || desc_.score_cap > 512.f;
+    a.series = !half || cap > 512.0;
+    const double by = !a.capped ? scale * log2e : a.series ? cap * log2e : 2.0 * cap * log2e;
+    a.by = (float)by;
+    a.to_slope = (float)(log2e / by);
+    a.in_cap = a.capped ? (float)(scale / cap * 2.0 * log2e) : 0.f;
     a.cell_x = desc_.cell_size[0];
     a.cell_y = desc_.cell_size[1];
     a.cell_z = desc_.cell_size[2];

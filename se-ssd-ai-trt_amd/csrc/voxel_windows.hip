@@ -9,7 +9,12 @@
 //   window_place   rows into the list
 //
 // No atomics in the first pass: all of a near window's rows would ask at one address, 24 ns each (627 rows of 16 000 in one window: 15 us).
-// Where a window count is beyond what LDS holds (kMostCounted), windows are small and tickets are given out by atomics:
+// Tensors of up to kFewRows rows take one launch instead of three, which is what bounds a call on few rows (the host takes 3.4 us for a launch):
+//
+//   window_few     kFewOwn rows a workgroup, and the windows of all rows in its LDS: a row's place is the number of rows with smaller windows and of
+//                  those with the same one in front of it.  (Comparisons bound it: 2 000 rows 12 us with 64 rows a workgroup, 6 with 16)
+//
+// Where a larger tensor has more windows than LDS holds counts for (kMostCounted), windows are small and tickets are given out by atomics:
 //
 //   window_ticket, window_base, window_scatter, window_rank    the last puts a window's rows in ascending order
 #include "fill.h"
@@ -21,16 +26,10 @@ namespace {
 
 constexpr int kBlock = 256;
 constexpr int kChunk = 1024;
+constexpr int kFewOwn = 16;
 constexpr int kMostCounted = 32768;  // windows: 64 KB of 16-bit counts
-constexpr int kLong = 128;           // rows of a window whose items come first: the last to end should not be the last to begin
 
 size_t counted_windows(size_t windows) { return (windows + 7) / 8 * 8; }
-
-// window of a row's voxel, -1 = outside the grid
-__device__ __forceinline__ int window_of(const int4 c, const WindowGrid& g) {  // (b,z,y,x)
-    if (c.x != 0 || c.y < 0 || c.y >= g.shape[0] || c.z < 0 || c.z >= g.shape[1] || c.w < 0 || c.w >= g.shape[2]) return -1;
-    return ((c.y + g.shift[0]) / g.window[0] * g.count[1] + (c.z + g.shift[1]) / g.window[1]) * g.count[2] + (c.w + g.shift[2]) / g.window[2];
-}
 
 __global__ void __launch_bounds__(kChunk)
 window_count(const int32_t* __restrict__ coors, const int32_t* __restrict__ voxel_num, WindowGrid g, int windows, int bits, WindowIndex w) {
@@ -89,9 +88,10 @@ window_base(const int32_t* __restrict__ voxel_num, int windows, int chunked, Win
         }
     }
     const int base = take(&w.head[kHeadPlaces], rows);
-    const int items = (rows + kItemRows - 1) / kItemRows;
-    const bool is_long = rows > kLong;
+    const int items = rows > kTinyRows ? (rows + kItemRows - 1) / kItemRows : 0;
+    const bool is_long = rows > kShortRows, is_tiny = rows > 0 && rows <= kTinyRows;
     const int front = take(&w.head[kHeadLong], is_long ? items : 0), back = take(&w.head[kHeadShort], is_long ? 0 : items);
+    const int tiny = take(&w.head[kHeadTiny], is_tiny ? 1 : 0);
     if (!rows) return;
     if (chunked) {
         int at = base;
@@ -103,12 +103,13 @@ window_base(const int32_t* __restrict__ voxel_num, int windows, int chunked, Win
     } else {
         w.base[i] = base;
     }
+    if (is_tiny) w.tiny[tiny] = make_int2(base, rows);
     for (int k = 0; k < items; ++k) w.items[is_long ? front + k : w.items_cap - 1 - (back + k)] = make_int4(base, rows, k * kItemRows, 0);
 }
 
-__device__ __forceinline__ void set_place(const WindowIndex& w, int place, int row, const int4 c) {
+__device__ __forceinline__ void set_place(const WindowIndex& w, const WindowGrid& g, int place, int row, const int4 c) {
     w.order[place] = row;
-    w.cell[place] = make_float4((float)c.w, (float)c.z, (float)c.y, 0.f);
+    w.cell[place] = cell_of(c, g);
 }
 __device__ __forceinline__ void set_outside(const WindowIndex& w, int n, int row) {
     w.order[n - 1 - atomicAdd(&w.head[kHeadOutside], 1)] = row;
@@ -116,15 +117,70 @@ __device__ __forceinline__ void set_outside(const WindowIndex& w, int n, int row
 }
 
 __global__ void __launch_bounds__(kBlock)
-window_place(const int32_t* __restrict__ coors, const int32_t* __restrict__ voxel_num, int windows, WindowIndex w) {
+window_place(const int32_t* __restrict__ coors, const int32_t* __restrict__ voxel_num, WindowGrid g, int windows, WindowIndex w) {
     const int row = blockIdx.x * kBlock + threadIdx.x;
     if (row >= w.max_voxels) return;
     const int4 c = reinterpret_cast<const int4*>(coors)[row];
     const int n = clamp_rows(voxel_num, w.max_voxels);
     if (row >= n) return;
     const int2 t = w.ticket[row];
-    if (t.x >= 0) set_place(w, w.chunk_base[(size_t)(row / kChunk) * windows + t.x] + t.y, row, c);
+    if (t.x >= 0) set_place(w, g, w.chunk_base[(size_t)(row / kChunk) * windows + t.x] + t.y, row, c);
     else set_outside(w, n, row);
+}
+
+__global__ void __launch_bounds__(1024)
+window_few(const int32_t* __restrict__ coors, const int32_t* __restrict__ voxel_num, WindowGrid g, WindowIndex w) {
+    constexpr int kOutside = 0x7fffffff;                  // behind all windows
+    __shared__ __align__(16) int32_t s_key[kFewRows];
+    __shared__ int32_t s_sum[16][3][kFewOwn];
+    __shared__ int32_t s_outside;
+    const int tid = threadIdx.x, wave = tid >> 6, mine_at = tid % kFewOwn, own = blockIdx.x * kFewOwn + mine_at;
+    const int n = clamp_rows(voxel_num, w.max_voxels), end = (n + 63) / 64 * 64;
+    if (tid == 0) s_outside = 0;
+    __syncthreads();
+    int outside = 0;
+    for (int i = tid; i < end; i += 1024) {
+        const int key = i < n ? window_of(reinterpret_cast<const int4*>(coors)[i], g) : -1;
+        s_key[i] = key < 0 ? kOutside : key;
+        outside += i < n && key < 0 ? 1 : 0;
+    }
+    if (blockIdx.x == 0 && outside) atomicAdd(&s_outside, outside);
+    __syncthreads();
+    if (blockIdx.x == 0 && tid == 0) {
+        w.head[kHeadStatus] = s_outside ? SESSD_STATUS_BAD_COORD : 0;
+        w.head[kHeadPlaces] = n - s_outside;
+    }
+    if ((int)blockIdx.x * kFewOwn >= n) return;
+    // (the rows between n and end are behind all others: smaller than none, equal to those outside, in front of none)
+    const int mine = own < n ? s_key[own] : kOutside;
+    int sum[3] = {0, 0, 0};                               // smaller ones, the same, those of them in front
+    for (int i = tid / kFewOwn * 4; i < end; i += 1024 / kFewOwn * 4) {
+        const int4 k = *reinterpret_cast<const int4*>(s_key + i);
+        sum[0] += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
+        const int e0 = k.x == mine, e1 = k.y == mine, e2 = k.z == mine, e3 = k.w == mine;
+        sum[1] += e0 + e1 + e2 + e3;
+        sum[2] += (i < own ? e0 : 0) + (i + 1 < own ? e1 : 0) + (i + 2 < own ? e2 : 0) + (i + 3 < own ? e3 : 0);
+    }
+#pragma unroll
+    for (int c = 0; c < 3; ++c) {
+#pragma unroll
+        for (int d = kFewOwn; d < 64; d *= 2) sum[c] += __shfl_xor(sum[c], d);
+        if ((tid & 63) < kFewOwn) s_sum[wave][c][mine_at] = sum[c];
+    }
+    __syncthreads();
+    if (tid >= kFewOwn || own >= n) return;
+    int less = 0, same = 0, before = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        less += s_sum[i][0][mine_at];
+        same += s_sum[i][1][mine_at];
+        before += s_sum[i][2][mine_at];
+    }
+    const int place = less + before;
+    w.order[place] = own;
+    if (mine == kOutside) return;
+    w.cell[place] = cell_of(reinterpret_cast<const int4*>(coors)[own], g);
+    w.span[place] = make_int2(less, same);
 }
 
 __global__ void __launch_bounds__(kBlock)
@@ -146,7 +202,7 @@ window_scatter(const int32_t* __restrict__ voxel_num, WindowIndex w) {
 }
 
 __global__ void __launch_bounds__(kBlock)
-window_rank(const int32_t* __restrict__ coors, WindowIndex w) {
+window_rank(const int32_t* __restrict__ coors, WindowGrid g, WindowIndex w) {
     const int p = blockIdx.x * kBlock + threadIdx.x;
     if (p >= w.head[kHeadPlaces]) return;
     const int row = w.list[p], key = w.ticket[row].x;
@@ -154,42 +210,46 @@ window_rank(const int32_t* __restrict__ coors, WindowIndex w) {
     int rank = 0;
 #pragma unroll 4
     for (int i = 0; i < rows; ++i) rank += w.list[start + i] < row ? 1 : 0;
-    set_place(w, start + rank, row, reinterpret_cast<const int4*>(coors)[row]);
+    set_place(w, g, start + rank, row, reinterpret_cast<const int4*>(coors)[row]);
 }
 
 }  // namespace
 
 WindowIndex carve_windows(void* workspace, int max_voxels, size_t windows) {
-    const bool counted = windows <= kMostCounted;
-    const size_t rows = (size_t)max_voxels, chunks = (rows + kChunk - 1) / kChunk;
+    const bool few = max_voxels <= kFewRows, counted = !few && windows <= kMostCounted, ticketed = !few && !counted;
+    const size_t rows = (size_t)max_voxels, listed = few ? 0 : rows, chunks = (listed + kChunk - 1) / kChunk;
     WorkspaceCarver c(workspace);
     WindowIndex w;
     w.max_voxels = max_voxels;
-    w.items_cap = (int32_t)((rows < windows ? rows : windows) + rows / kItemRows);
+    w.items_cap = (int32_t)(rows / (kTinyRows + 1) + rows / kItemRows) + 1;  // (windows that have items, and whole items)
     w.head = c.take<int32_t>(kHeadWords);
     w.order = c.take<int32_t>(rows);
     w.cell = c.take<float4>(rows);
-    w.items = c.take<int4>((size_t)w.items_cap);
-    w.ticket = c.take<int2>(rows);
+    w.span = c.take<int2>(few ? rows : 0);
+    w.items = c.take<int4>(few ? 0 : (size_t)w.items_cap);
+    w.tiny = c.take<int2>(listed < windows ? listed : windows);
+    w.ticket = c.take<int2>(listed);
     w.chunk_count = c.take<uint16_t>(counted ? chunks * counted_windows(windows) : 0);
     w.chunk_base = c.take<int32_t>(counted ? chunks * counted_windows(windows) : 0);
-    w.list = c.take<int32_t>(counted ? 0 : rows);
-    w.count = c.take<int32_t>(counted ? 0 : windows);
-    w.base = c.take<int32_t>(counted ? 0 : windows);
+    w.list = c.take<int32_t>(ticketed ? rows : 0);
+    w.count = c.take<int32_t>(ticketed ? windows : 0);
+    w.base = c.take<int32_t>(ticketed ? windows : 0);
     w.bytes = c.total();
     return w;
 }
 
 int launch_windows(const int32_t* coors, const int32_t* voxel_num, const WindowGrid& g, const WindowIndex& w, hipStream_t stream) {
     const dim3 rows((unsigned)ceil_div(w.max_voxels, kBlock)), block(kBlock);
-    if (g.windows() <= kMostCounted) {
+    if (w.max_voxels <= kFewRows) {
+        hipLaunchKernelGGL(window_few, dim3((unsigned)ceil_div(w.max_voxels, kFewOwn)), dim3(1024), 0, stream, coors, voxel_num, g, w);
+    } else if (g.windows() <= kMostCounted) {
         const int windows = (int)counted_windows(g.windows());
         int bits = 0;
         while (((size_t)1 << bits) < g.windows()) ++bits;
         hipLaunchKernelGGL(window_count, dim3((unsigned)ceil_div(w.max_voxels, kChunk)), dim3(kChunk), (size_t)windows * sizeof(uint16_t), stream, coors,
                            voxel_num, g, windows, bits, w);
         hipLaunchKernelGGL(window_base, dim3((unsigned)ceil_div(windows, kBlock)), block, 0, stream, voxel_num, windows, 1, w);
-        hipLaunchKernelGGL(window_place, rows, block, 0, stream, coors, voxel_num, windows, w);
+        hipLaunchKernelGGL(window_place, rows, block, 0, stream, coors, voxel_num, g, windows, w);
     } else {
         const int windows = (int)g.windows();
         FillArgs f;
@@ -199,7 +259,7 @@ int launch_windows(const int32_t* coors, const int32_t* voxel_num, const WindowG
         hipLaunchKernelGGL(window_ticket, rows, block, 0, stream, coors, voxel_num, g, w);
         hipLaunchKernelGGL(window_base, dim3((unsigned)ceil_div(windows, kBlock)), block, 0, stream, voxel_num, windows, 0, w);
         hipLaunchKernelGGL(window_scatter, rows, block, 0, stream, voxel_num, w);
-        hipLaunchKernelGGL(window_rank, rows, block, 0, stream, coors, w);
+        hipLaunchKernelGGL(window_rank, rows, block, 0, stream, coors, g, w);
     }
     SESSD_HIP_TRY(hipGetLastError());
     return SESSD_OK;

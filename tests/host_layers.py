@@ -190,12 +190,11 @@ def check_attention():
         refused(conf(i, o), code, "voxelattn")
     i, o = descs(*ATT_IN), descs(*ATT_OUT)
     size = L.sessd_voxelattn_workspace_size(h, i, 3, o, 1)
-    assert 100 * 4 < size < 1 << 20
+    assert 0 < size < 1 << 20
     a, b = pointers(4096, 8192, 12292), pointers(16384)
-    for call, some in ((L.sessd_voxelattn_enqueue, True), (L.sessd_voxelattn_enqueue_shared, False)):
+    for call, n in ((L.sessd_voxelattn_enqueue, 2), (L.sessd_voxelattn_enqueue_shared, 1)):
         assert call(h, i, o, a, b, 65536, None) == 0
-        n = len(launches())
-        assert n > 1 if some else n == 1
+        assert len(launches()) == n
         for v, w, ws in (((4104, 8192, 64), 16384, 65536), ((4096, 8200, 64), 16384, 65536), ((4096, 8192, 64), 16386, 65536), ((0, 8192, 64), 16384, 65536),
                          ((4096, 0, 64), 16384, 65536), ((4096, 8192, 0), 16384, 65536), ((4096, 8192, 64), 0, 65536), ((4096, 8192, 64), 16384, 0),
                          ((4096, 8192, 64), 16384, 65544)):
@@ -203,6 +202,15 @@ def check_attention():
         refused(call(h, descs(*both(F32)[0]), descs(*both(F32)[1]), a, b, 65536, None), E, "configured")
         refused(call(None, i, o, a, b, 65536, None), E)
     L.sessd_voxelattn_destroy(h)
+    # a list of the rows by windows where there are many, from counts or from tickets; layers that share it need none
+    for grid, window, own in ((GRID, WINDOW, 4), ((1000, 1000, 1), (2, 2, 1), 6)):
+        h = attention(rows=5000, grid=grid, window=window)[1]
+        i, o = descs(((1, 5000, 128), F16), ((1, 5000, 4), I32), ((1,), I32)), descs(((1, 5000, 64), F16))
+        assert L.sessd_voxelattn_configure(h, i, 3, o, 1) == 0
+        for call, n in ((L.sessd_voxelattn_enqueue, own), (L.sessd_voxelattn_enqueue_shared, 1)):
+            assert call(h, i, o, a, b, 65536, None) == 0
+            assert len(launches()) == n
+        L.sessd_voxelattn_destroy(h)
 
 
 def blob_of(name, h):

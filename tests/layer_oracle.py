@@ -79,8 +79,9 @@ def attention(qkv, coors, n, grid_zyx, window_zyx, shift_zyx, heads, kv_heads, d
     beyond n: zeros.
 
     The bound.  A score t = scale * q.k is within e_t = (dim + 2) u * scale * sum|q_d k_d| of itself, which the cap's slope (at most 1)
-    does not enlarge; the cap itself adds 8 u * cap (argument, exponential, quotient, product), the distance 8 u * slope * |p_i - p_j|
-    (three differences exact, squares, sums, root, product).  Taken to the base 2 and less the maximum, it is rounded three times
+    does not enlarge; the cap itself adds 8 u * cap (argument, exponential, quotient, product).  A voxel's place is taken from its
+    window's first cell on and is within u of itself, so that a difference is within 2 u * extent of the window on that axis and a
+    distance within 4 u * the extents' sum and, for squares, sums, root and product, 8 u of itself.  Taken to the base 2 and less the maximum, it is rounded three times
     more: 4 u * (|t| + |max|).  With e the largest such error of a row, a weight is within 2 e + 8 u of itself relative to the
     others (2^x within 4 u), the sum of L weights and that of L products within L u each, every rescaling of a running sum
     by 8 u more, L / 32 of them at most.  FP16: the weights are rounded to 11 bits, relative 2^-11 or 2^-25 of the largest weight.
@@ -94,6 +95,7 @@ def attention(qkv, coors, n, grid_zyx, window_zyx, shift_zyx, heads, kv_heads, d
     inside = (c[:, 0] == 0) & (c[:, 1:] >= 0).all(1) & (c[:, 1:] < grid).all(1) if n else np.zeros(0, bool)
     win = (c[:, 1:] + np.array(shift_zyx)) // np.array(window_zyx)
     p_at = c[:, 1:] * np.array(cell_zyx, np.float32).astype(np.float64)
+    extent = float((np.minimum(window_zyx, grid) * np.abs(np.array(cell_zyx, np.float64))).sum())
     at = np.nonzero(inside)[0]
     if not len(at):
         return out, bound
@@ -114,7 +116,7 @@ def attention(qkv, coors, n, grid_zyx, window_zyx, shift_zyx, heads, kv_heads, d
                     e = e + 8 * U * cap
                 if slopes is not None:
                     t = t - float(slopes[h]) * far
-                    e = e + 8 * U * abs(float(slopes[h])) * far
+                    e = e + abs(float(slopes[h])) * (8 * U * far + 4 * U * extent)
                 e = (e + 4 * U * (np.abs(t) + np.abs(t.max(1, keepdims=True)))).max(1, keepdims=True)
                 p = np.exp(t - t.max(1, keepdims=True))
                 total = p.sum(1, keepdims=True)

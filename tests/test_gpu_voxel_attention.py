@@ -48,12 +48,21 @@ class Case:
         assert not off.any(), (int(off.sum()), np.argwhere(off)[:3], float((np.abs(g - want) / tol)[off].max()))
 
 
+MANY = 4200  # rows of a tensor whose windows are listed; those of smaller ones are looked up by the attention itself
+
+
 def run(case, rows, n, dtype, **kw):
+    """The rows as they are, and at the front of a large tensor."""
     qkv, coors = make(rows, case.heads, case.kv, case.dim, dtype, **kw)
-    op = case.op(rows)
-    got = op(dev(qkv), dev(coors), num(n))
-    case.check(got, qkv, coors, n)
-    assert op.status() == 0
+    for more in (0, MANY):
+        if more:
+            n = min(max(n, 0), rows)
+            qkv = np.concatenate([qkv, np.full((more, qkv.shape[1]), np.nan, qkv.dtype)])
+            coors = np.concatenate([coors, np.full((more, 4), -1, np.int32)])
+        op = case.op(rows + more)
+        got = op(dev(qkv), dev(coors), num(n))
+        case.check(got, qkv, coors, n)
+        assert op.status() == 0
     return got
 
 
@@ -72,10 +81,18 @@ def test_rows_and_windows(rows, n, dtype, window):
     run(Case(4, 2, 16, window, slopes=[1, 2, 3, 4]), rows, n, dtype)
 
 
+@pytest.mark.parametrize("rows,n,window", [(5000, 5000, (2, 2, 2)), (6000, 5900, (21, 30, 44)), (9000, 9000, (1, 1, 1)), (4097, 4097, (3, 5, 4))])
+@pytest.mark.parametrize("dtype", [HALF, FLOAT])
+def test_grids_of_many_windows(rows, n, window, dtype):
+    """Up to 2^22 windows, and window counts either side of what is counted in LDS."""
+    grid = (21, 300, 220)
+    run(Case(2, 2, 16, window, slopes=[1.0, 0.5], grid=grid), rows, n, dtype, grid=grid)
+
+
 @pytest.mark.parametrize("shift", [(0, 0, 0), (1, 0, 0), (0, 3, 5), (2, 6, 6), (1, 1, 1)])
 @pytest.mark.parametrize("dtype", [HALF, FLOAT])
 def test_shifted_windows(shift, dtype):
-    run(Case(2, 2, 32, (3, 7, 7), shift=shift), 1500, 1500, dtype)
+    run(Case(2, 2, 32, (3, 7, 7), shift=shift, slopes=[1.0, 0.25]), 1500, 1500, dtype)
 
 
 @pytest.mark.parametrize("cap,slopes,scale", [(0.0, None, 0.0), (5.0, None, 0.0), (0.0, [2.0, -1.0], 0.0), (50.0, [0.0, 0.3], 0.5), (1000.0, None, -0.3), (0.01, [30.0, 1.0], 4.0)])
@@ -116,58 +133,61 @@ def test_long_windows_of_ragged_lengths():
 
 
 @pytest.mark.parametrize("dtype", [HALF, FLOAT])
-@pytest.mark.parametrize("window", [(9, 2, 2), (9, 20, 25)])
-def test_what_is_not_finite_stays_in_its_window(dtype, window):
+@pytest.mark.parametrize("window", [(9, 2, 2), (9, 4, 5), (9, 20, 25)])
+@pytest.mark.parametrize("rows", [1200, MANY])
+def test_what_is_not_finite_stays_in_its_window(dtype, window, rows):
     case = Case(2, 1, 16, window, slopes=[1.0, 0.5], cap=10.0)
-    qkv, coors = make(1200, 2, 1, 16, dtype)
-    op = case.op(1200)
+    qkv, coors = make(rows, 2, 1, 16, dtype)
+    op = case.op(rows)
     clean = op(dev(qkv), dev(coors), num(1150))
-    rows = (3, 400, 777)
-    for row, bad in zip(rows, (np.nan, np.inf, -np.inf)):
+    bad_rows = (3, 400, 777)
+    for row, bad in zip(bad_rows, (np.nan, np.inf, -np.inf)):
         qkv[row] = bad
     qkv[1150:] = np.nan     # rows behind the last
     coors[1150:] = -7
     got = op(dev(qkv), dev(coors), num(1150))
     win = coors[:1150, 1:] // np.array(window)
-    touched = np.zeros(1200, bool)
-    for row in rows:
+    touched = np.zeros(rows, bool)
+    for row in bad_rows:
         touched[:1150] |= (win == win[row]).all(1)
     assert touched.sum() < 1150
     assert torch.equal(got[dev(~touched)], clean[dev(~touched)])
     # in the window of the NaN every row has it among its keys; what inf leaves is the formula's affair
-    mine = np.zeros(1200, bool)
+    mine = np.zeros(rows, bool)
     mine[:1150] = (win == win[3]).all(1)
     assert torch.isnan(got[dev(mine)]).all()
 
 
 @pytest.mark.parametrize("dtype", [HALF, FLOAT])
-def test_a_row_outside_the_grid_takes_part_in_nothing(dtype):
+@pytest.mark.parametrize("rows", [300, MANY])
+def test_a_row_outside_the_grid_takes_part_in_nothing(dtype, rows):
     case = Case(2, 2, 16, (9, 40, 50))
-    qkv, coors = make(300, 2, 2, 16, dtype)
+    qkv, coors = make(rows, 2, 2, 16, dtype)
     coors[5] = (0, 9, 0, 0)
     coors[17] = (0, 0, -1, 3)
     coors[18] = (1, 0, 1, 3)
     coors[299] = (0, 2 ** 31 - 1, -2 ** 31, 50)
     qkv[[5, 17, 18, 299]] = np.nan
-    op = case.op(300)
+    op = case.op(rows)
     op.set_flags(D.SESSD_FLAG_SKIP_PAD_ROWS)
-    got = op(dev(qkv), dev(coors), num(300))
-    case.check(got, qkv, coors, 300)
+    got = op(dev(qkv), dev(coors), num(300))[:300]  # (the rows behind it are anything)
+    case.check(got, qkv[:300], coors, 300)
     assert not got[[5, 17, 18, 299]].any() and op.status() == D.SESSD_STATUS_BAD_COORD
     coors[:, 0] = 3         # every row
-    assert not op(dev(qkv), dev(coors), num(300)).any()
+    assert not op(dev(qkv), dev(coors), num(300))[:300].any()
     coors[:, 0] = 0
     coors[[5, 17, 299], 1:] = 1
     op(dev(np.nan_to_num(qkv)), dev(coors), num(300))
     assert op.status() == 0
 
 
-def test_rows_behind_the_last_are_left_as_they_were():
+@pytest.mark.parametrize("rows", [200, MANY])
+def test_rows_behind_the_last_are_left_as_they_were(rows):
     case = Case(2, 2, 24, (9, 8, 8))
-    qkv, coors = make(200, 2, 2, 24, HALF)
-    op = case.op(200)
+    qkv, coors = make(rows, 2, 2, 24, HALF)
+    op = case.op(rows)
     op.set_flags(D.SESSD_FLAG_SKIP_PAD_ROWS)
-    out = torch.full((200, 48), 7.0, dtype=HALF, device=DEV)
+    out = torch.full((rows, 48), 7.0, dtype=HALF, device=DEV)
     ins = [dev(qkv), dev(coors), num(131)]
     op.configure(ins, [out])
     op.enqueue(ins, [out])
@@ -180,23 +200,24 @@ def test_rows_behind_the_last_are_left_as_they_were():
 
 @pytest.mark.parametrize("dtype", [HALF, FLOAT])
 @pytest.mark.parametrize("window", [(9, 5, 5), (9, 40, 50)])
-def test_the_same_bits_each_time_and_on_shared_windows(dtype, window):
+@pytest.mark.parametrize("rows", [2500, 5000])
+def test_the_same_bits_each_time_and_on_shared_windows(dtype, window, rows):
     case = Case(8, 4, 32, window, slopes=np.linspace(0, 2, 8), cap=25.0)
-    qkv, coors = make(5000, 8, 4, 32, dtype)
-    x, c, n = dev(qkv), dev(coors), num(4900)
-    first, second = case.op(5000), case.op(5000)
+    qkv, coors = make(rows, 8, 4, 32, dtype)
+    x, c, n = dev(qkv), dev(coors), num(rows - 100)
+    first, second = case.op(rows), case.op(rows)
     a = first(x, c, n)
     for _ in range(3):
         assert torch.equal(first(x, c, n), a)
     assert torch.equal(second(x, c, n, windows_from=first), a)
     other = Case(2, 2, 16, window)    # another layer on the same windows
-    qkv2, _ = make(5000, 2, 2, 16, dtype)
-    assert torch.equal(other.op(5000)(dev(qkv2), c, n, windows_from=first), other.op(5000)(dev(qkv2), c, n))
+    qkv2, _ = make(rows, 2, 2, 16, dtype)
+    assert torch.equal(other.op(rows)(dev(qkv2), c, n, windows_from=first), other.op(rows)(dev(qkv2), c, n))
     # a row's bits follow from its window's rows, wherever else rows lie: the rows of the other windows leave
     if window == (9, 5, 5):
-        keep = (coors[:4900, 3] // 5) % 2 == 0
+        keep = (coors[:rows - 100, 3] // 5) % 2 == 0
         got = first(x, dev(np.where(np.concatenate([keep, np.ones(100, bool)])[:, None], coors, -1).astype(np.int32)), n)
-        assert torch.equal(got[:4900][dev(keep)], a[:4900][dev(keep)])
+        assert torch.equal(got[:rows - 100][dev(keep)], a[:rows - 100][dev(keep)])
 
 
 def test_order_of_rows_does_not_choose_neighbours():
@@ -211,26 +232,28 @@ def test_order_of_rows_does_not_choose_neighbours():
     assert np.abs(a[p] - b).max() < 1e-4
 
 
-def test_dirty_workspace_and_outputs():
+@pytest.mark.parametrize("rows", [600, MANY])
+def test_dirty_workspace_and_outputs(rows):
     case = Case(2, 2, 16, (9, 6, 6), slopes=[1, 2])
-    qkv, coors = make(600, 2, 2, 16, HALF)
-    op = case.op(600)
+    qkv, coors = make(rows, 2, 2, 16, HALF)
+    op = case.op(rows)
     ins = [dev(qkv), dev(coors), num(555)]
     for fill in (0xff, 0x7f, 0x01):
-        out = torch.full((600, 32), float("nan"), dtype=HALF, device=DEV)
+        out = torch.full((rows, 32), float("nan"), dtype=HALF, device=DEV)
         op.configure(ins, [out])
         ws = torch.full((op.workspace_size(ins, [out]),), fill, dtype=torch.uint8, device=DEV)
         op.enqueue(ins, [out], workspace=ws)
         case.check(out, qkv, coors, 555)
 
 
-def test_two_calls_at_once():
+@pytest.mark.parametrize("rows", [4000, 8000])
+def test_two_calls_at_once(rows):
     """Two layers on two streams, each with a workspace of its own."""
     case = Case(4, 4, 16, (9, 8, 8), slopes=[1, 1, 2, 2])
-    qkv, coors = make(4000, 4, 4, 16, HALF)
-    qkv2, coors2 = make(4000, 4, 4, 16, HALF, seed=9)
-    a, b = case.op(4000), case.op(4000)
-    one, two = (dev(qkv), dev(coors), num(3900)), (dev(qkv2), dev(coors2), num(4000))
+    qkv, coors = make(rows, 4, 4, 16, HALF)
+    qkv2, coors2 = make(rows, 4, 4, 16, HALF, seed=9)
+    a, b = case.op(rows), case.op(rows)
+    one, two = (dev(qkv), dev(coors), num(rows - 100)), (dev(qkv2), dev(coors2), num(rows))
     want = a(*one).clone(), b(*two).clone()
     s, t = torch.cuda.Stream(), torch.cuda.Stream()
     torch.cuda.synchronize()
@@ -265,12 +288,13 @@ def test_rows_beyond_32_bit_offsets():
     assert not got[:-n].any()
 
 
-def test_under_a_graph():
+@pytest.mark.parametrize("rows", [1500, MANY])
+def test_under_a_graph(rows):
     case = Case(4, 2, 16, (9, 8, 8), slopes=[1, 1, 2, 2], cap=20.0)
-    qkv, coors = make(1500, 4, 2, 16, HALF)
+    qkv, coors = make(rows, 4, 2, 16, HALF)
     x, c, n = dev(qkv), dev(coors), num(1400)
-    op, eager_op = case.op(1500), case.op(1500)
-    out = torch.empty((1500, 64), dtype=HALF, device=DEV)
+    op, eager_op = case.op(rows), case.op(rows)
+    out = torch.empty((rows, 64), dtype=HALF, device=DEV)
     eager = torch.empty_like(out)
     ws = torch.empty(op.workspace_size([x, c, n], [out]), dtype=torch.uint8, device=DEV)
     for o in (op, eager_op):
@@ -282,8 +306,8 @@ def test_under_a_graph():
         op.enqueue([x, c, n], [out], side, workspace=ws)
     rng = np.random.default_rng(0)
     for k in range(4):
-        m = (1400, 1500, 3, 700)[k]
-        p = rng.permutation(1500)
+        m = (1400, rows, 3, 700)[k]
+        p = rng.permutation(rows)
         x.copy_(dev(qkv[p]))
         c.copy_(dev(coors[p]))
         n.copy_(num(m))
