@@ -332,14 +332,14 @@ void sessd_sparse2dense_destroy(sessd_sparse2dense* h);
  * bits, the projection that reads such rows, and attention among the voxels of a window.  Life cycle, tensors, streams
  * and errors are those of the layers above; the first two need no workspace (workspace_size is 0, NULL is accepted).
  * Rows beyond voxel_num: zeros, or what Linear8's epilogue makes of zeros; left as they were with
- * SESSD_FLAG_SKIP_PAD_ROWS. */
+ * SESSD_FLAG_SKIP_PAD_ROWS.  max_voxels: up to 2^24.  Outputs must not overlap inputs, but for RmsNorm's sum. */
 
 /* inputs : 0 feat [1,max_voxels,C] f32|f16   1 voxel_num i32[1]   [2 residual, as feat]
  * outputs: 0 q fp8 [1,max_voxels,C]   1 scale f32 [1,max_voxels,1]   [2 sum, as feat]
  * h = feat + residual, y = gamma * h / sqrt(mean over C of h^2 + eps), scale = max(max|y| / 448, 2^-100),
  * q = y / scale to the nearest e4m3, sum = h.  All of it is computed in FP32 from the unrounded h.  A row with a value
  * that is not finite, or whose mean of h^2 is not (|h| from about 1e19), leaves nothing that counts: its scale is NaN and
- * all of its q are.  `sum` may be the tensor `feat` or `residual`; no other output may overlap an input.
+ * all of its q are.  `sum` may be the tensor `feat` or `residual`.
  * With two inputs there are two outputs, with three three.  channel: 1 .. 4096, multiples of 8 are fastest. */
 typedef struct sessd_rmsnorm sessd_rmsnorm;
 

@@ -31,8 +31,9 @@ constexpr int tiles_of(int cin) { return cin > 256 && cin <= kMostHeld ? 2 : 4; 
 // Rows and weights meet in 64 input channels at a time, two instructions: lane group g has 16 neighbouring channels of each row, 8 to either
 constexpr int pairs_of(int cin) { return (cin + 63) / 64; }
 constexpr int channel_of(int step, int g, int e) { return step / 2 * 64 + g * 16 + step % 2 * 8 + e; }
-// column that row `i` of instruction `t` stands for: lane group g (rows 4 g .. 4 g + 3) gets 4 NT neighbouring ones over the NT
-constexpr int column_of(int tiles, int t, int i) { return 4 * tiles * (i / 4) + 4 * t + i % 4; }
+// Column that row `i` of instruction `t` stands for: a lane (its group g has rows 4 g .. 4 g + 3) gets 16 bytes of neighbouring columns from each
+// instruction in FP32 and from each two in FP16, and the four groups of a store 64 bytes of a row
+constexpr int column_of(bool half, int t, int i) { return half ? 32 * (t / 2) + 8 * (i / 4) + 4 * (t % 2) + i % 4 : 16 * t + i; }
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
@@ -55,40 +56,53 @@ struct LinearArgs {
     void* out;
 };
 
-// 4 NT neighbouring columns of a row, from `c0` on
+// (past the caches: 150 000 x 256 -> 1024 150 us through them, 107 like this)
+template <typename V>
+__device__ __forceinline__ void put(V* to, const V& x) {
+    __builtin_nontemporal_store(x, to);
+}
+
+// A lane's 4 NT columns of a row, of the block of columns from `c0` on
 template <typename T, int NT>
-__device__ __forceinline__ void store_columns(const LinearArgs& a, int row, int c0, const v4f (&acc)[NT], float s, const v4f* factor, const v4f* addend) {
-    float y[4 * NT];
+__device__ __forceinline__ void store_columns(const LinearArgs& a, int row, int c0, const v4f (&acc)[NT], float s, const float* factor, const float* addend, int g) {
+    constexpr bool kHalf = sizeof(T) == 2;
+    T* const dst = static_cast<T*>(a.out) + (size_t)row * a.cout + c0;
+    const bool whole = a.cout % (16 / (int)sizeof(T)) == 0 && c0 + 16 * NT <= a.cout;
+    float y[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const v4f f = factor[t], b = addend[t];
+        const int c = column_of(kHalf, t, 4 * g);
+        const v4f f = *reinterpret_cast<const v4f*>(factor + c), b = *reinterpret_cast<const v4f*>(addend + c);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float x = fmaf(acc[t][e] * s, f[e], b[e]);
-            y[4 * t + e] = a.relu && x < 0.f ? 0.f : x;
-        }
+        for (int e = 0; e < 4; ++e) y[t][e] = fmaf(acc[t][e] * s, f[e], b[e]);
     }
-    T* dst = static_cast<T*>(a.out) + (size_t)row * a.cout + c0;
-    constexpr int kPer = 16 / (int)sizeof(T);
-    if (a.cout % kPer == 0 && c0 + 4 * NT <= a.cout) {
+    if (a.relu) {
 #pragma unroll
-        for (int i = 0; i < 4 * NT / kPer; ++i) {
-            if constexpr (sizeof(T) == 2) {
-                v8h x;
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = (_Float16)y[8 * i + e];
-                reinterpret_cast<v8h*>(dst)[i] = x;
-            } else {
-                reinterpret_cast<v4f*>(dst)[i] = v4f{y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]};
+            for (int e = 0; e < 4; ++e) y[t][e] = y[t][e] < 0.f ? 0.f : y[t][e];
+    }
+    if (!whole) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int c = column_of(kHalf, t, 4 * g) + e;
+                if (c0 + c >= a.cout) continue;
+                if constexpr (kHalf) dst[c] = __float2half_rn(y[t][e]);
+                else dst[c] = y[t][e];
             }
+    } else if constexpr (kHalf) {
+#pragma unroll
+        for (int t = 0; t < NT; t += 2) {
+            v8h x;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = (_Float16)y[t + e / 4][e % 4];
+            put(reinterpret_cast<v8h*>(dst + column_of(true, t, 4 * g)), x);
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 4 * NT; ++e)
-            if (c0 + e < a.cout) {
-                if constexpr (sizeof(T) == 2) dst[e] = __float2half_rn(y[e]);
-                else dst[e] = y[e];
-            }
+        for (int t = 0; t < NT; ++t) put(reinterpret_cast<v4f*>(dst + column_of(false, t, 4 * g)), v4f{y[t][0], y[t][1], y[t][2], y[t][3]});
     }
 }
 
@@ -97,39 +111,49 @@ template <typename T, int PAIRS, int NT>
 __global__ void __launch_bounds__(kBlock, 2)
 linear8_held(LinearArgs a) {
     constexpr int kWide = 16 * NT;
-    __shared__ v4f s_columns[kBlock / 64][2][kWide / 4];
+    __shared__ __align__(16) float s_columns[kBlock / 64][2][kWide];
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
-    const int blocks = (a.cout + kWide - 1) / kWide, id = (int)blockIdx.x * (kBlock / 64) + wave;
+    // (workgroups go to the eight dies in turn: neighbours in rows and columns on one of them)
+    const int group = gridDim.x % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
+    const int blocks = (a.cout + kWide - 1) / kWide, id = group * (kBlock / 64) + wave;
     const int cb = id % blocks, stream = id / blocks, streams = (int)gridDim.x * (kBlock / 64) / blocks;
     if (stream >= streams) return;  // (what is left over; no wave waits for another)
-    const int pairs = (a.cin + 63) / 64;
     v8h w[2 * PAIRS][NT];
-    const v8h* from = reinterpret_cast<const v8h*>(a.w) + (size_t)cb * 2 * pairs * NT * 64 + lane;
+    const v8h* from = reinterpret_cast<const v8h*>(a.w) + (size_t)cb * 2 * PAIRS * NT * 64 + lane;
 #pragma unroll
     for (int s = 0; s < 2 * PAIRS; ++s)
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-            if (s < 2 * pairs) w[s][t] = from[(s * NT + t) * 64];
-    if (lane < kWide / 4)
+        for (int t = 0; t < NT; ++t) w[s][t] = from[(s * NT + t) * 64];
+    if (lane < kWide)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) s_columns[wave][i][lane] = reinterpret_cast<const v4f*>(a.columns + i * blocks * kWide + cb * kWide)[lane];
+        for (int i = 0; i < 2; ++i) s_columns[wave][i][lane] = a.columns[i * blocks * kWide + cb * kWide + lane];
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     const int n = clamp_rows(a.voxel_num, a.max_voxels), rows = a.write_pad ? a.max_voxels : n;
     v4u x[PAIRS];
-    float scale = 0.f;
-    const auto request = [&](int row) {  // a row's values, zeros behind the last one
-        scale = 0.f;
-        if (row < n) scale = a.scale[row];
+    float scale;
+    const bool whole = a.cin % 64 == 0;
+    // 16 rows' values, zeros behind the last one (for most blocks without a branch, which each load would wait in front of)
+    const auto request = [&](int first) {
+        const uint8_t* const at = a.q + (size_t)(first + r) * a.cin + g * 16;
+        if (whole && first + kRows <= n) {
+            scale = a.scale[first + r];
 #pragma unroll
-        for (int p = 0; p < PAIRS; ++p) {
-            x[p] = v4u{0, 0, 0, 0};
-            if (row < n && p * 64 + g * 16 < a.cin) x[p] = *reinterpret_cast<const v4u*>(a.q + (size_t)row * a.cin + p * 64 + g * 16);
+            for (int p = 0; p < PAIRS; ++p) x[p] = *reinterpret_cast<const v4u*>(at + p * 64);
+        } else {
+            scale = 0.f;
+            if (first + r < n) scale = a.scale[first + r];
+#pragma unroll
+            for (int p = 0; p < PAIRS; ++p) {
+                x[p] = v4u{0, 0, 0, 0};
+                if (first + r < n && p * 64 + g * 16 < a.cin) x[p] = *reinterpret_cast<const v4u*>(at + p * 64);
+            }
         }
     };
-    request(stream * kRows + r);
-    for (int row0 = stream * kRows; row0 < rows; row0 += streams * kRows) {
+    const int turn = streams * kRows;
+    request(stream * kRows);
+    for (int first = stream * kRows; first < rows; first += turn) {
         v8h b[2 * PAIRS];
 #pragma unroll
         for (int p = 0; p < PAIRS; ++p) {
@@ -137,15 +161,13 @@ linear8_held(LinearArgs a) {
             b[2 * p + 1] = widen(x[p][2], x[p][3]);
         }
         const float s = scale;
-        request(row0 + streams * kRows + r);
+        request(first + turn);
         v4f acc[NT] = {};
 #pragma unroll
         for (int k = 0; k < 2 * PAIRS; ++k)
-            if (k < 2 * pairs) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[k][t], b[k], acc[t], 0, 0, 0);
-            }
-        if (row0 + r < rows) store_columns<T, NT>(a, row0 + r, cb * kWide + 4 * NT * g, acc, s, s_columns[wave][0] + NT * g, s_columns[wave][1] + NT * g);
+            for (int t = 0; t < NT; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[k][t], b[k], acc[t], 0, 0, 0);
+        if (first + r < rows) store_columns<T, NT>(a, first + r, cb * kWide, acc, s, s_columns[wave][0], s_columns[wave][1], g);
     }
 }
 
@@ -169,9 +191,7 @@ linear8_wide(LinearArgs a) {
         }
     }
     if (row >= a.max_voxels || (row >= n && !a.write_pad)) return;
-    const int c0 = cb * kWide + 4 * NT * g;
-    const v4f* columns = reinterpret_cast<const v4f*>(a.columns + c0);
-    store_columns<T, NT>(a, row, c0, acc, row < n ? a.scale[row] : 0.f, columns, columns + blocks * kWide / 4);
+    store_columns<T, NT>(a, row, cb * kWide, acc, row < n ? a.scale[row] : 0.f, a.columns + cb * kWide, a.columns + (blocks + cb) * kWide, g);
 }
 
 template <typename T>
@@ -188,7 +208,11 @@ void launch_linear8(const LinearArgs& a, hipStream_t stream) {
     switch (pairs_of(a.cin)) {
         case 1: SESSD_HELD(1, 4); break;
         case 2: SESSD_HELD(2, 4); break;
-        case 3: case 4: SESSD_HELD(4, 4); break;
+        case 3: SESSD_HELD(3, 4); break;
+        case 4: SESSD_HELD(4, 4); break;
+        case 5: SESSD_HELD(5, 2); break;
+        case 6: SESSD_HELD(6, 2); break;
+        case 7: SESSD_HELD(7, 2); break;
         default: SESSD_HELD(8, 2); break;
     }
 #undef SESSD_HELD
@@ -215,9 +239,9 @@ Linear8Plugin::~Linear8Plugin() {
 int Linear8Plugin::create(const sessd_linear8_desc& d, const float* weights, Linear8Plugin** out) {
     if (d.in_channel < 1 || d.out_channel < 1 || d.max_voxels < 1)
         return fail(SESSD_E_INVALID, "linear8: in_channel, out_channel and max_voxels must be positive");
-    if (d.in_channel % 16 || d.in_channel > 4096 || d.out_channel > 4096)
-        return fail(SESSD_E_UNSUPPORTED, "linear8: in_channel must be a multiple of 16 up to 4096, out_channel at most 4096 (%d, %d)",
-                    d.in_channel, d.out_channel);
+    if (d.in_channel % 16 || d.in_channel > 4096 || d.out_channel > 4096 || d.max_voxels > kMostRows)
+        return fail(SESSD_E_UNSUPPORTED, "linear8: in_channel must be a multiple of 16 up to 4096, out_channel at most 4096, max_voxels at most %d (%d, %d, %d)",
+                    kMostRows, d.in_channel, d.out_channel, d.max_voxels);
     const int cin = d.in_channel, cout = d.out_channel;
     for (size_t i = 0; i < (size_t)cin * cout; ++i)
         if (!std::isfinite(weights[i])) return fail(SESSD_E_INVALID, "linear8: the weights must be finite");
@@ -231,20 +255,24 @@ int Linear8Plugin::create(const sessd_linear8_desc& d, const float* weights, Lin
         for (int c = 0; c < cout; ++c) p->wscale_[c] = std::fmax(p->wscale_[c], std::fabs(weights[(size_t)k * cout + c]));
     for (float& s : p->wscale_) s = std::fmax(s / 448.f, 0x1p-100f);
     const int tiles = tiles_of(cin), steps = 2 * pairs_of(cin), blocks = padded_columns(cin, cout) / (16 * tiles);
-    std::vector<uint16_t> packed((size_t)blocks * steps * tiles * 64 * 8, 0);
-    for (int cb = 0; cb < blocks; ++cb)
-        for (int s = 0; s < steps; ++s)
-            for (int t = 0; t < tiles; ++t)
-                for (int lane = 0; lane < 64; ++lane) {
-                    const int c = cb * 16 * tiles + column_of(tiles, t, lane & 15);
-                    uint16_t* dst = packed.data() + ((((size_t)cb * steps + s) * tiles + t) * 64 + lane) * 8;
-                    for (int e = 0; e < 8; ++e) {
-                        const int k = channel_of(s, lane >> 4, e);
-                        if (c < cout && k < cin) dst[e] = nearest_e4m3(weights[(size_t)k * cout + c] / p->wscale_[c]);
+    const size_t count = (size_t)blocks * steps * tiles * 64 * 8;
+    std::vector<uint16_t> packed(count);
+    SESSD_HIP_TRY(hipMalloc(reinterpret_cast<void**>(&p->weights_packed_dev_), 2 * count * sizeof(uint16_t)));
+    for (const bool half : {false, true}) {  // (the order of the columns is the output's)
+        for (int cb = 0; cb < blocks; ++cb)
+            for (int s = 0; s < steps; ++s)
+                for (int t = 0; t < tiles; ++t)
+                    for (int lane = 0; lane < 64; ++lane) {
+                        const int c = cb * 16 * tiles + column_of(half, t, lane & 15);
+                        uint16_t* dst = packed.data() + ((((size_t)cb * steps + s) * tiles + t) * 64 + lane) * 8;
+                        for (int e = 0; e < 8; ++e) {
+                            const int k = channel_of(s, lane >> 4, e);
+                            dst[e] = c < cout && k < cin ? nearest_e4m3(weights[(size_t)k * cout + c] / p->wscale_[c]) : 0;
+                        }
                     }
-                }
-    SESSD_HIP_TRY(hipMalloc(reinterpret_cast<void**>(&p->weights_packed_dev_), packed.size() * sizeof(uint16_t)));
-    SESSD_HIP_TRY(hipMemcpy(p->weights_packed_dev_, packed.data(), packed.size() * sizeof(uint16_t), hipMemcpyHostToDevice));
+        SESSD_HIP_TRY(hipMemcpy(p->weights_packed_dev_ + (half ? count : 0), packed.data(), count * sizeof(uint16_t), hipMemcpyHostToDevice));
+    }
+    p->packed_count_ = count;
     SESSD_TRY(p->uploadColumns());
     *out = p.release();
     return SESSD_OK;
@@ -348,7 +376,7 @@ int Linear8Plugin::enqueue(const sessd_tensor_desc* inputDesc, const sessd_tenso
     a.cout = out_channel_;
     a.relu = epi_.relu;
     a.write_pad = (flags_ & SESSD_FLAG_SKIP_PAD_ROWS) ? 0 : 1;
-    a.w = weights_packed_dev_;
+    a.w = weights_packed_dev_ + (out_type_ == SESSD_HALF ? packed_count_ : 0);
     a.columns = columns_dev_;
     a.out = outputs[0];
     if (out_type_ == SESSD_HALF) launch_linear8<__half>(a, stream);

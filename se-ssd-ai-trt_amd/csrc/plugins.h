@@ -318,7 +318,8 @@ class Linear8Plugin {
 
     int in_channel_ = 0, out_channel_ = 0, max_voxels_ = 0;
     std::vector<float> weights_;         // as given, FP32 [Cin][Cout]
-    __half* weights_packed_dev_ = nullptr;  // e4m3 values as halves, operand order (linear8.hip)
+    __half* weights_packed_dev_ = nullptr;  // e4m3 values as halves, operand order (linear8.hip): for FP32 outputs, for FP16 ones
+    size_t packed_count_ = 0;            // of either
     float* columns_dev_ = nullptr;       // factor and addend of each column (linear8.hip)
     Epilogue epi_;                       // (host side; the device has it in columns_dev_)
     int out_type_ = SESSD_FLOAT;
@@ -358,7 +359,9 @@ class VoxelAttentionPlugin {
     int attend(const void* const* inputs, void* const* outputs, const void* workspace, hipStream_t stream) const;
 };
 
-// Tensors of these layers: [1, max_voxels, channels]; the scalars in device memory
+// Tensors of these layers: [1, max_voxels, channels]; the scalars in device memory.  (Rows, items of an attention and lanes of a launch are
+// counted in 32 bits.)
+constexpr int kMostRows = 1 << 24;
 int check_rows(const sessd_tensor_desc& d, int max_voxels, int channels, const char* who, const char* what);
 bool is_scalar_int(const sessd_tensor_desc& d);
 

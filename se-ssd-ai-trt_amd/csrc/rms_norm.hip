@@ -230,7 +230,8 @@ RmsNormPlugin::~RmsNormPlugin() {
 
 int RmsNormPlugin::create(const sessd_rmsnorm_desc& d, const float* gamma, RmsNormPlugin** out) {
     if (d.channel < 1 || d.max_voxels < 1) return fail(SESSD_E_INVALID, "rmsnorm: channel and max_voxels must be positive");
-    if (d.channel > 4096) return fail(SESSD_E_UNSUPPORTED, "rmsnorm: channel %d is beyond 4096", d.channel);
+    if (d.channel > 4096 || d.max_voxels > kMostRows)
+        return fail(SESSD_E_UNSUPPORTED, "rmsnorm: at most 4096 channels and %d rows (%d, %d)", kMostRows, d.channel, d.max_voxels);
     if (!(d.eps >= 0.f) || !std::isfinite(d.eps)) return fail(SESSD_E_INVALID, "rmsnorm: eps must be finite and not negative");
     for (int i = 0; i < d.channel; ++i)
         if (!std::isfinite(gamma[i])) return fail(SESSD_E_INVALID, "rmsnorm: gamma must be finite");

@@ -43,9 +43,9 @@ int VoxelAttentionPlugin::create(const sessd_voxelattn_desc& d, const float* slo
     if (d.num_heads < 1 || d.num_kv_heads < 1 || d.head_dim < 1 || d.max_voxels < 1)
         return fail(SESSD_E_INVALID, "voxelattn: heads, head_dim and max_voxels must be positive");
     if (d.num_heads % d.num_kv_heads) return fail(SESSD_E_INVALID, "voxelattn: num_heads must be a multiple of num_kv_heads");
-    if (d.head_dim % 8 || d.head_dim > 128 || d.num_heads > 1024)
-        return fail(SESSD_E_UNSUPPORTED, "voxelattn: head_dim must be a multiple of 8 up to 128, num_heads at most 1024 (%d, %d)", d.head_dim,
-                    d.num_heads);
+    if (d.head_dim % 8 || d.head_dim > 128 || d.num_heads > 1024 || d.max_voxels > kMostRows)
+        return fail(SESSD_E_UNSUPPORTED, "voxelattn: head_dim must be a multiple of 8 up to 128, num_heads at most 1024, max_voxels at most %d (%d, %d, %d)", kMostRows,
+                    d.head_dim, d.num_heads, d.max_voxels);
     for (int a = 0; a < 3; ++a) {
         if (d.spatial_shape[a] < 1 || d.window_shape[a] < 1 || d.window_shift[a] < 0 || d.window_shift[a] >= d.window_shape[a])
             return fail(SESSD_E_INVALID, "voxelattn: shapes must be positive, shifts 0 .. window_shape - 1");

@@ -14,7 +14,8 @@
 //   window_few     kFewOwn rows a workgroup, and the windows of all rows in its LDS: a row's place is the number of rows with smaller windows and of
 //                  those with the same one in front of it.  (Comparisons bound it: 2 000 rows 12 us with 64 rows a workgroup, 6 with 16)
 //
-// Where a larger tensor has more windows than LDS holds counts for (kMostCounted), windows are small and tickets are given out by atomics:
+// Where a larger tensor has more windows than LDS holds counts for (kMostCounted), windows are small, and where it has more than 2^20 rows, tickets
+// are given out by atomics:
 //
 //   window_ticket, window_base, window_scatter, window_rank    the last puts a window's rows in ascending order
 #include "fill.h"
@@ -28,6 +29,9 @@ constexpr int kBlock = 256;
 constexpr int kChunk = 1024;
 constexpr int kFewOwn = 16;
 constexpr int kMostCounted = 32768;  // windows: 64 KB of 16-bit counts
+
+constexpr int kMostCountedRows = 1 << 20;  // 1 024 chunks, whose counts a thread adds up
+bool counts(int max_voxels, size_t windows) { return windows <= kMostCounted && max_voxels <= kMostCountedRows; }
 
 size_t counted_windows(size_t windows) { return (windows + 7) / 8 * 8; }
 
@@ -216,7 +220,7 @@ window_rank(const int32_t* __restrict__ coors, WindowGrid g, WindowIndex w) {
 }  // namespace
 
 WindowIndex carve_windows(void* workspace, int max_voxels, size_t windows) {
-    const bool few = max_voxels <= kFewRows, counted = !few && windows <= kMostCounted, ticketed = !few && !counted;
+    const bool few = max_voxels <= kFewRows, counted = !few && counts(max_voxels, windows), ticketed = !few && !counted;
     const size_t rows = (size_t)max_voxels, listed = few ? 0 : rows, chunks = (listed + kChunk - 1) / kChunk;
     WorkspaceCarver c(workspace);
     WindowIndex w;
@@ -242,7 +246,7 @@ int launch_windows(const int32_t* coors, const int32_t* voxel_num, const WindowG
     const dim3 rows((unsigned)ceil_div(w.max_voxels, kBlock)), block(kBlock);
     if (w.max_voxels <= kFewRows) {
         hipLaunchKernelGGL(window_few, dim3((unsigned)ceil_div(w.max_voxels, kFewOwn)), dim3(1024), 0, stream, coors, voxel_num, g, w);
-    } else if (g.windows() <= kMostCounted) {
+    } else if (counts(w.max_voxels, g.windows())) {
         const int windows = (int)counted_windows(g.windows());
         int bits = 0;
         while (((size_t)1 << bits) < g.windows()) ++bits;

@@ -455,6 +455,13 @@ class Sparse2Dense(_Plugin):
         return int(self.ws[:4].view(torch.int32)[0].item())
 
 
+def _dense(*tensors):
+    """The library reads and writes rows one behind the other: views with other strides are refused."""
+    for t in tensors:
+        if not t.is_contiguous():
+            raise SessdError("a tensor is not contiguous: shape %s, strides %s" % (tuple(t.shape), t.stride()))
+
+
 class RmsNorm(_Plugin):
     """h = feat + residual; gamma * h / sqrt(mean(h^2) + eps) in e4m3 with a scale for each row."""
     kind = "rmsnorm"
@@ -471,12 +478,12 @@ class RmsNorm(_Plugin):
     def __call__(self, feat, voxel_num, residual=None, stream=None):
         """feat, residual [max_voxels, channel] -> q float8_e4m3fn, scale f32 [max_voxels, 1] (, sum as feat, with a residual)"""
         torch = _torch()
-        q = feat.new_empty((self.max_voxels, self.channel), dtype=torch.float8_e4m3fn)
-        scale = feat.new_empty((self.max_voxels, 1), dtype=torch.float32)
-        if residual is None:
-            ins, outs = (feat, voxel_num), (q, scale)
-        else:
-            ins, outs = (feat, voxel_num, residual), (q, scale, feat.new_empty((self.max_voxels, self.channel)))
+        ins = (feat, voxel_num) if residual is None else (feat, voxel_num, residual)
+        _dense(*ins)
+        # (outputs like feat: where that has another shape than the layer, configure says so)
+        outs = (torch.empty_like(feat, dtype=torch.float8_e4m3fn), feat.new_empty((self.max_voxels, 1), dtype=torch.float32))
+        if residual is not None:
+            outs += (torch.empty_like(feat),)
         self._enqueue_bound(self._bound_configured(ins, outs), ins, outs, stream)
         return outs
 
@@ -502,8 +509,10 @@ class Linear8(_Plugin):
 
     def __call__(self, q, scale, voxel_num, out_dtype=None, stream=None):
         """q float8_e4m3fn [max_voxels, in_channel], scale f32 [max_voxels, 1] -> [max_voxels, out_channel], FP16 unless said otherwise"""
+        ins = (q, scale, voxel_num)
+        _dense(*ins)
         out = q.new_empty((self.max_voxels, self.cout), dtype=out_dtype or _torch().float16)
-        ins, outs = (q, scale, voxel_num), (out,)
+        outs = (out,)
         self._enqueue_bound(self._bound_configured(ins, outs), ins, outs, stream)
         return out
 
@@ -530,8 +539,10 @@ class VoxelAttention(_Plugin):
     def __call__(self, qkv, coors, voxel_num, stream=None, windows_from=None):
         """qkv [max_voxels, (num_heads + 2 num_kv_heads) * head_dim] -> [max_voxels, num_heads * head_dim].  windows_from: a layer on
         the same coordinates and windows that has run on this stream."""
+        ins = (qkv, coors, voxel_num)
+        _dense(*ins)
         out = qkv.new_empty((self.max_voxels, self.cout))
-        ins, outs = (qkv, coors, voxel_num), (out,)
+        outs = (out,)
         bound = self._bound_configured(ins, outs)
         if windows_from is None:
             self._enqueue_bound(bound, ins, outs, stream)

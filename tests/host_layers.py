@@ -65,15 +65,15 @@ def attention(heads=4, kv=2, dim=16, rows=100, grid=GRID, window=WINDOW, shift=(
 
 def check_create():
     E, U = D.SESSD_E_INVALID, D.SESSD_E_UNSUPPORTED
-    for kw, code in ((dict(channel=0), E), (dict(channel=-4), E), (dict(rows=0), E), (dict(channel=4097), U), (dict(eps=-1.0), E),
+    for kw, code in ((dict(channel=0), E), (dict(channel=-4), E), (dict(rows=0), E), (dict(channel=4097), U), (dict(rows=(1 << 24) + 1), U), (dict(eps=-1.0), E),
                      (dict(eps=float("nan")), E), (dict(eps=float("inf")), E), (dict(gamma=[1.0] * 47 + [float("nan")]), E)):
         refused(norm(**kw)[0], code, "rmsnorm")
     bad = np.ones((32, 20))
     bad[3, 4] = np.inf
     for kw, code in ((dict(cin=0), E), (dict(cin=-16), E), (dict(cout=0), E), (dict(rows=-1), E), (dict(cin=24), U), (dict(cin=4112), U),
-                     (dict(cout=4097), U), (dict(w=bad), E)):
+                     (dict(cout=4097), U), (dict(rows=(1 << 24) + 1), U), (dict(w=bad), E)):
         refused(linear(**kw)[0], code, "linear8")
-    for kw, code in ((dict(heads=0), E), (dict(kv=0), E), (dict(heads=4, kv=3), E), (dict(dim=0), E), (dict(dim=12), U), (dict(dim=136), U),
+    for kw, code in ((dict(heads=0), E), (dict(kv=0), E), (dict(heads=4, kv=3), E), (dict(dim=0), E), (dict(dim=12), U), (dict(dim=136), U), (dict(rows=(1 << 24) + 1), U),
                      (dict(rows=0), E), (dict(heads=2048, kv=2048), U), (dict(window=(0, 8, 8)), E), (dict(shift=(8, 0, 0)), E),
                      (dict(shift=(0, -1, 0)), E), (dict(grid=(70, 0, 10)), E), (dict(grid=(1 << 25, 1, 1), window=(1 << 20, 1, 1)), U),
                      (dict(grid=(4096, 1024, 2), window=(1, 1, 1)), U), (dict(grid=(1 << 24, 1 << 24, 1 << 24), window=(1, 1, 1)), U),

@@ -300,3 +300,26 @@ def test_layers_under_a_graph_and_on_another_stream():
         if k == 0:
             for x, y in zip(eager, other):
                 assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+def test_wrong_tensors_are_refused():
+    f = torch.randn(64, 100, device=DEV).half()
+    norm = api.RmsNorm(100, np.ones(100, np.float32), max_voxels=64)
+    with pytest.raises(api.SessdError, match="contiguous"):
+        norm(torch.randn(100, 64, device=DEV).half().t(), num(64))
+    with pytest.raises(api.SessdError, match="feat must be"):
+        norm(f[:, :96].contiguous(), num(64))
+    with pytest.raises(api.SessdError, match="feat must be"):
+        norm(f[:63], num(63))
+    with pytest.raises(api.SessdError, match="type"):
+        norm(f, num(64), f.float())
+    with pytest.raises(api.SessdError, match="aligned"):
+        norm(torch.randn(6401, device=DEV).half()[1:].reshape(64, 100), num(64))
+    lin = api.Linear8(32, 16, np.ones((32, 16), np.float32), max_voxels=64)
+    q, s = torch.zeros(64, 32, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn), torch.ones(64, 1, device=DEV)
+    for bad in ((q[:, :16].contiguous(), s, num(1)), (q, s.expand(64, 2), num(1)), (q, s, num(1).float()), (f, s, num(1)), (q, s.half(), num(1))):
+        with pytest.raises(api.SessdError):
+            lin(*bad)
+    with pytest.raises(api.SessdError, match="FP32 or FP16"):
+        lin(q, s, num(1), out_dtype=torch.float8_e4m3fn)
+    assert torch.equal(lin(q, s, num(64)), torch.zeros(64, 16, dtype=HALF, device=DEV))
