@@ -533,7 +533,7 @@ voxel_attention(AttentionArgs a) {
 
 // The same where the list has spans (few rows): kFewPlaces places and a head are a workgroup's, which takes the tiny windows that begin
 // among them and the blocks of 64 queries that do.
-constexpr int kFewPlaces = 32;
+constexpr int kFewPlaces = 16;
 template <typename S, int CAP, bool BIAS>
 __global__ void __launch_bounds__(kAttentionBlock, 2)
 voxel_attention_few(AttentionArgs a) {

@@ -12,7 +12,7 @@
 // Tensors of up to kFewRows rows take one launch instead of three, which is what bounds a call on few rows (the host takes 3.4 us for a launch):
 //
 //   window_few     kFewOwn rows a workgroup, and the windows of all rows in its LDS: a row's place is the number of rows with smaller windows and of
-//                  those with the same one in front of it.  (Comparisons bound it: 2 000 rows 12 us with 64 rows a workgroup, 6 with 16)
+//                  those with the same one in front of it.  (Comparisons bound it: 2 000 rows 12 us with 64 rows a workgroup, 6 with 16, 5 with 8)
 //
 // Where a larger tensor has more windows than LDS holds counts for (kMostCounted), windows are small, and where it has more than 2^20 rows, tickets
 // are given out by atomics:
@@ -27,7 +27,7 @@ namespace {
 
 constexpr int kBlock = 256;
 constexpr int kChunk = 1024;
-constexpr int kFewOwn = 16;
+constexpr int kFewOwn = 8;
 constexpr int kMostCounted = 32768;  // windows: 64 KB of 16-bit counts
 
 constexpr int kMostCountedRows = 1 << 20;  // 1 024 chunks, whose counts a thread adds up
@@ -69,40 +69,60 @@ window_count(const int32_t* __restrict__ coors, const int32_t* __restrict__ voxe
     for (int i = threadIdx.x; i < windows / 8; i += kChunk) dst[i] = s_count4[i];
 }
 
-// place `mine` of this lane behind those of the lanes before it, in a range of the list that the wave takes
-__device__ __forceinline__ int take(int32_t* from, int mine) {
-    const uint32_t upto = wave_scan((uint32_t)mine);
-    int at = 0;
-    if (lane_id() == 63 && upto) at = atomicAdd(from, (int)upto);
-    return __shfl(at, 63) + (int)upto - mine;
-}
+constexpr int kTaken = 4;  // ranges that window_base takes: places, long items, short items, tiny windows
 
-// chunks 0: the counts are w.count's, and the bases go to w.base
-__global__ void __launch_bounds__(kBlock)
-window_base(const int32_t* __restrict__ voxel_num, int windows, int chunked, WindowIndex w) {
-    const int i = blockIdx.x * kBlock + threadIdx.x;
-    const int chunks = chunked ? (clamp_rows(voxel_num, w.max_voxels) + kChunk - 1) / kChunk : 0;
+// Windows of a workgroup of window_base.  A workgroup takes its ranges with one atomic each, 8 ns apiece where all ask at one address: 250 000 windows
+// 34 us with an atomic for each wave, 5 us with one for 1 024 windows.  Where chunks are to be added up, smaller workgroups reach more of the card.
+constexpr int kBaseCounted = 256, kBaseTicketed = 1024;
+
+template <bool CHUNKED, int BLOCK>
+__global__ void __launch_bounds__(BLOCK)
+window_base(const int32_t* __restrict__ voxel_num, int windows, WindowIndex w) {
+    constexpr int kWaves = BLOCK / 64;
+    __shared__ int32_t s_sum[kWaves][kTaken], s_from[kTaken];
+    const int i = blockIdx.x * BLOCK + threadIdx.x, wave = threadIdx.x >> 6;
+    const int chunks = CHUNKED ? (clamp_rows(voxel_num, w.max_voxels) + kChunk - 1) / kChunk : 0;
     int rows = 0;
     if (i < windows) {
-        if (chunked) {
+        if constexpr (CHUNKED) {
 #pragma unroll 8
             for (int c = 0; c < chunks; ++c) rows += w.chunk_count[(size_t)c * windows + i];
         } else {
             rows = w.count[i];
         }
     }
-    const int base = take(&w.head[kHeadPlaces], rows);
     const int items = rows > kTinyRows ? (rows + kItemRows - 1) / kItemRows : 0;
     const bool is_long = rows > kShortRows, is_tiny = rows > 0 && rows <= kTinyRows;
-    const int front = take(&w.head[kHeadLong], is_long ? items : 0), back = take(&w.head[kHeadShort], is_long ? 0 : items);
-    const int tiny = take(&w.head[kHeadTiny], is_tiny ? 1 : 0);
+    const int mine[kTaken] = {rows, is_long ? items : 0, is_long ? 0 : items, is_tiny ? 1 : 0};
+    int at[kTaken];
+#pragma unroll
+    for (int k = 0; k < kTaken; ++k) {
+        const int upto = (int)wave_scan((uint32_t)mine[k]);
+        at[k] = upto - mine[k];
+        if (lane_id() == 63) s_sum[wave][k] = upto;
+    }
+    __syncthreads();
+    if (threadIdx.x < kTaken) {
+        int all = 0;
+#pragma unroll
+        for (int v = 0; v < kWaves; ++v) {
+            const int sum = s_sum[v][threadIdx.x];
+            s_sum[v][threadIdx.x] = all;
+            all += sum;
+        }
+        s_from[threadIdx.x] = all ? atomicAdd(&w.head[kHeadPlaces + threadIdx.x], all) : 0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kTaken; ++k) at[k] += s_sum[wave][k] + s_from[k];
+    const int base = at[0], front = at[1], back = at[2], tiny = at[3];
     if (!rows) return;
-    if (chunked) {
-        int at = base;
+    if constexpr (CHUNKED) {
+        int next = base;
 #pragma unroll 8
         for (int c = 0; c < chunks; ++c) {
-            w.chunk_base[(size_t)c * windows + i] = at;
-            at += w.chunk_count[(size_t)c * windows + i];
+            w.chunk_base[(size_t)c * windows + i] = next;
+            next += w.chunk_count[(size_t)c * windows + i];
         }
     } else {
         w.base[i] = base;
@@ -252,7 +272,8 @@ int launch_windows(const int32_t* coors, const int32_t* voxel_num, const WindowG
         while (((size_t)1 << bits) < g.windows()) ++bits;
         hipLaunchKernelGGL(window_count, dim3((unsigned)ceil_div(w.max_voxels, kChunk)), dim3(kChunk), (size_t)windows * sizeof(uint16_t), stream, coors,
                            voxel_num, g, windows, bits, w);
-        hipLaunchKernelGGL(window_base, dim3((unsigned)ceil_div(windows, kBlock)), block, 0, stream, voxel_num, windows, 1, w);
+        hipLaunchKernelGGL((window_base<true, kBaseCounted>), dim3((unsigned)ceil_div(windows, kBaseCounted)), dim3(kBaseCounted), 0, stream, voxel_num,
+                           windows, w);
         hipLaunchKernelGGL(window_place, rows, block, 0, stream, coors, voxel_num, g, windows, w);
     } else {
         const int windows = (int)g.windows();
@@ -261,7 +282,8 @@ int launch_windows(const int32_t* coors, const int32_t* voxel_num, const WindowG
         f.add(w.count, (uint64_t)windows, 0);
         SESSD_TRY(launch_fill(f, stream));
         hipLaunchKernelGGL(window_ticket, rows, block, 0, stream, coors, voxel_num, g, w);
-        hipLaunchKernelGGL(window_base, dim3((unsigned)ceil_div(windows, kBlock)), block, 0, stream, voxel_num, windows, 0, w);
+        hipLaunchKernelGGL((window_base<false, kBaseTicketed>), dim3((unsigned)ceil_div(windows, kBaseTicketed)), dim3(kBaseTicketed), 0, stream, voxel_num,
+                           windows, w);
         hipLaunchKernelGGL(window_scatter, rows, block, 0, stream, voxel_num, w);
         hipLaunchKernelGGL(window_rank, rows, block, 0, stream, coors, g, w);
     }
