@@ -401,7 +401,8 @@ void sessd_linear8_destroy(sessd_linear8* h);
  * Scores, softmax and sums are FP32; with FP16 tensors the weights are rounded to FP16 in front of their product with v.
  * A row whose coordinates lie outside the grid takes part in nothing, its output is zeros and SESSD_STATUS_BAD_COORD is
  * raised.  Rows that name one voxel are all of them rows of its window.  No value of another window reaches a row, whatever
- * it is.  The order of a row's sums follows from the window's rows alone: ascending. */
+ * it is.  The order of a row's sums follows from its window's rows, ascending, and the layer's own sizes: a row's bits do not
+ * depend on the other windows. */
 typedef struct sessd_voxelattn sessd_voxelattn;
 
 typedef struct sessd_voxelattn_desc {

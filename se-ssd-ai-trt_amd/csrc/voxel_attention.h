@@ -3,7 +3,8 @@
 // A workgroup of four waves takes up to 64 queries of one window and a few heads, and walks over the window's keys in blocks of 64 (32
 // where a head's values are many).  Keys, values and voxels of a block lie in LDS; those of the next one are gathered into registers in
 // the meantime.  A wave has 16 queries; where the window has fewer than 64, waves share queries and deal the heads out.  Windows of up to
-// 32 rows are a wave's own affair: their queries are their keys, which it keeps in registers, and nobody waits for anybody.
+// 32 rows are a wave's own affair: their queries are their keys, which it keeps in registers, and nobody waits for anybody.  Where there are
+// few queries, a workgroup has 16 of them and its waves share the keys out (shared_rows).
 //
 // Scores are taken transposed, S^T = K Q^T: a lane of the result has one query (its column) and four keys, so that maximum and sum over the
 // keys are mostly the lane's own, and the weights are where the second product, O^T = V^T P^T, wants them.  Maximum and sum run along
@@ -206,6 +207,9 @@ struct AttentionShape {
     static constexpr int kTiny = kAttentionBlock / 64 * kTinyRows * Op::kPitch;          // the values of a tiny window for each wave
     static constexpr int kWordsHead = DP / Op::kPer;                                     // 16-byte words of a head's row
     static constexpr int kLoads = (2 * KVG * kWordsHead * KB + kAttentionBlock - 1) / kAttentionBlock;  // of a thread
+    // Where the waves of a workgroup share the keys out: keys of a wave's block (up to eight words of a lane), its keys and values in LDS
+    static constexpr int KW = 256 / kWordsHead > 64 ? 64 : 256 / kWordsHead < 16 ? 16 : 256 / kWordsHead;
+    static constexpr int kWave = 2 * KW * Op::kPitch;
 };
 
 enum { kCapNone, kCapExponential, kCapSeries };
@@ -482,6 +486,117 @@ __device__ __forceinline__ void window_rows(const AttentionArgs& a, int start, i
         if (i < mine) store_row<S>(a, q_row, h_first + h0 + i, total[i], acc[i], q_there, g);
 }
 
+// Up to 16 queries of a window from q0 on and a head, by the workgroup: its waves have every fourth block of KW keys each, wait for nobody, and join
+// their sums at the end.  s_part: kWave elements of a wave, s_cell: KW of a wave.
+template <typename S, int CAP, bool BIAS>
+__device__ __forceinline__ void shared_rows(const AttentionArgs& a, int start, int len, int q0, int head, typename S::Type* s_part, float4* s_cell) {
+    using T = typename S::Type;
+    using Op = typename S::Op;
+    constexpr int KW = S::KW, DP = S::kDim, kWaves = kAttentionBlock / 64, kStep = 32 / S::kWordsHead, kLoads = KW / kStep;
+    constexpr int kJoin = DP + 4;  // floats of a query: sums, maximum, sum of the weights
+    static_assert(16 * kJoin * sizeof(float) <= S::kWave * sizeof(T), "a wave's sums lie where its keys were");
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const T* const qkv = static_cast<const T*>(a.qkv);
+    const int kv = head / (a.heads / a.kv_heads);
+    const size_t stride = (size_t)(a.heads + 2 * a.kv_heads) * a.dim;
+    const int32_t* const order = a.w.order + start;
+    const float4* const cells = a.w.cell + start;
+    T* const s_k = s_part + wave * S::kWave;
+    float4* const s_far = s_cell + wave * KW;
+
+    // words of a block: key by key, the key's and then the value's.  A lane has the same ones of every kStep-th key
+    const int first_key = lane / (2 * S::kWordsHead), half = lane / S::kWordsHead & 1, d = lane % S::kWordsHead * Op::kPer;
+    const T* const source = qkv + (size_t)(a.heads + kv + half * a.kv_heads) * a.dim + (d < a.dim ? d : 0);
+    T* const target = s_k + half * KW * Op::kPitch + first_key * Op::kPitch + d;
+    const auto row_of = [&](int k0) { return order[k0 + lane < len ? k0 + lane : len - 1]; };  // of the key lane of a block
+    v4u word[kLoads];
+    const auto gather = [&](int row, int left) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const unsigned at = (unsigned)__shfl(row, first_key + i * kStep);
+            word[i] = *reinterpret_cast<const v4u*>(source + (size_t)at * stride);
+            if (d >= a.dim || first_key + i * kStep >= left) word[i] = v4u{0, 0, 0, 0};
+        }
+    };
+    int k0 = wave * KW;
+    int row = row_of(k0);
+    const bool q_there = q0 + r < len;
+    const int q_row = order[q_there ? q0 + r : len - 1];
+    float4 cell = make_float4(0, 0, 0, 0), me = cell;
+    if (BIAS) {
+        cell = cells[k0 + lane < len ? k0 + lane : len - 1];
+        me = place_of(a, cells[q_there ? q0 + r : len - 1]);
+    }
+    gather(row, len - k0);
+    row = row_of(k0 + kWaves * KW);
+    const typename Op::Row q = load_query<S>(a, qkv + (size_t)(unsigned)q_row * stride, head, g);
+    const float slope = BIAS ? a.slopes[head] * a.to_slope : 0.f;
+    float most = -INFINITY;
+    typename Op::Sum total = {};
+    v4f acc[DP / 16] = {};
+    __syncthreads();  // (the item before is worked on)
+#pragma unroll 1
+    for (; k0 < len; k0 += kWaves * KW) {
+        const int left = len - k0;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) *reinterpret_cast<v4u*>(target + i * kStep * Op::kPitch) = word[i];
+        if (BIAS && lane < KW) s_far[lane] = place_of(a, cell);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (left > kWaves * KW) {  // the next block, and the rows of the one behind it
+            gather(row, left - kWaves * KW);
+            if (BIAS) cell = cells[kWaves * KW + lane < left ? k0 + kWaves * KW + lane : len - 1];
+            row = row_of(k0 + 2 * kWaves * KW);
+        }
+        const auto keys = [&](auto tail) {
+            constexpr int H = KW / 16;
+            float far[H][4];
+            v4f z[H];
+#pragma unroll
+            for (int t = 0; t < H; ++t) {
+                if constexpr (BIAS) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) far[t][e] = distance(s_far[16 * t + 4 * g + e], me);
+                }
+                z[t] = Op::scores(s_k + 16 * t * Op::kPitch, q, r, g);
+            }
+            attend<S, CAP, BIAS, H, decltype(tail)::value>(a, z, s_k + KW * Op::kPitch, far, slope, left, most, total, acc, r, g);
+        };
+        if (left >= KW) keys(std::false_type{});
+        else keys(std::true_type{});
+        __builtin_amdgcn_wave_barrier();
+    }
+    float* const s_join = reinterpret_cast<float*>(s_k) + r * kJoin;
+    const float sum = Op::sum(total);
+#pragma unroll
+    for (int b = 0; b < DP / 16; ++b) *reinterpret_cast<v4f*>(s_join + 16 * b + 4 * g) = acc[b];
+    if (g == 0) {
+        s_join[DP] = most;
+        s_join[DP + 1] = sum;
+    }
+    __syncthreads();
+    const auto of_wave = [&](int w) { return reinterpret_cast<const float*>(s_part + w * S::kWave) + r * kJoin; };
+    float all_most = -INFINITY, all = 0.f, by[kWaves];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) all_most = fmaxf(all_most, of_wave(w)[DP]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        by[w] = of_wave(w)[DP] == all_most ? 1.f : __builtin_amdgcn_exp2f((of_wave(w)[DP] - all_most) * a.by);
+        all = fmaf(of_wave(w)[DP + 1], by[w], all);
+    }
+    const float over = 1.f / all;
+    T* const dst = static_cast<T*>(a.out) + ((size_t)(unsigned)q_row * a.heads + head) * a.dim;
+#pragma unroll
+    for (int b = 0; b < DP / 16; ++b) {
+        if (b % kWaves != wave) continue;
+        v4f x = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) x += *reinterpret_cast<const v4f*>(of_wave(w) + 16 * b + 4 * g) * by[w];
+        if (q_there && 16 * b + 4 * g < a.dim) Op::store(dst + 16 * b + 4 * g, x * over);
+    }
+}
+
 template <typename S, int CAP, bool BIAS>
 __global__ void __launch_bounds__(kAttentionBlock, 2)
 voxel_attention(AttentionArgs a) {
@@ -532,16 +647,21 @@ voxel_attention(AttentionArgs a) {
 }
 
 // The same where the list has spans (few rows): kFewPlaces places and a head are a workgroup's, which takes the tiny windows that begin
-// among them and the blocks of 64 queries that do.
+// among them and the blocks of 64 queries (16, SHARED) that do.
 constexpr int kFewPlaces = 16;
-template <typename S, int CAP, bool BIAS>
+// Waves that share a query's keys reach four times as much of the card with few queries, but read each key for 16 queries instead of 64 and have more
+// registers.  FP16, 64 and 16 queries a workgroup: 1 951 rows of one window and 2 heads of 16 values 45 and 21 us, 4 096 and 8 of 64 415 and 193, but 24 of
+// 64 430 and 520, and windows of 60 rows at 4 096 rows and 16 heads 28 and 40.  FP32, whose products take longer: 4 096 rows and 16 heads of 64 1 509 and 936.
+constexpr int kSharedRows = 32768;  // rows times heads, FP16
+template <typename S, int CAP, bool BIAS, bool SHARED>
 __global__ void __launch_bounds__(kAttentionBlock, 2)
 voxel_attention_few(AttentionArgs a) {
     using T = typename S::Type;
     using Op = typename S::Op;
-    __shared__ __align__(16) T s_kv[2 * S::kHalf > S::kTiny ? 2 * S::kHalf : S::kTiny];
-    __shared__ float4 s_cell[S::KB];
-    __shared__ int32_t s_row[S::KB];
+    constexpr int kWaves = kAttentionBlock / 64, kKeys = SHARED ? kWaves * S::kWave : 2 * S::kHalf, kQueries = SHARED ? 16 : kItemRows;
+    __shared__ __align__(16) T s_kv[kKeys > S::kTiny ? kKeys : S::kTiny];
+    __shared__ float4 s_cell[SHARED ? kWaves * S::KW : S::KB];
+    __shared__ int32_t s_row[SHARED ? 1 : S::KB];
     T* const out = static_cast<T*>(a.out);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int first = (int)(blockIdx.x / (unsigned)a.heads) * kFewPlaces, head = (int)(blockIdx.x % (unsigned)a.heads);
@@ -550,10 +670,11 @@ voxel_attention_few(AttentionArgs a) {
     const bool there = lane < kFewPlaces && place < places;
     const int2 span = there ? a.w.span[place] : make_int2(0, 0);  // (every wave has all of them)
     const int before = place - span.x;
-    for (uint64_t m = __ballot(there && span.y > kTinyRows && before % kItemRows == 0); m; m &= m - 1) {
-        const int who = __builtin_ctzll(m);
-        window_rows<S, CAP, BIAS>(a, __builtin_amdgcn_readlane(span.x, who), __builtin_amdgcn_readlane(span.y, who), __builtin_amdgcn_readlane(before, who), head, 1,
-                                  s_kv, s_cell, s_row);
+    for (uint64_t m = __ballot(there && span.y > kTinyRows && before % kQueries == 0); m; m &= m - 1) {
+        const int who = __builtin_ctzll(m), start = __builtin_amdgcn_readlane(span.x, who), len = __builtin_amdgcn_readlane(span.y, who);
+        const int q0 = __builtin_amdgcn_readlane(before, who);
+        if constexpr (SHARED) shared_rows<S, CAP, BIAS>(a, start, len, q0, head, s_kv, s_cell);
+        else window_rows<S, CAP, BIAS>(a, start, len, q0, head, 1, s_kv, s_cell, s_row);
     }
     __syncthreads();  // (the last item is worked on)
     int turn = 0;
@@ -577,7 +698,12 @@ template <typename S, int CAP, bool BIAS>
 void launch_attention_as(const AttentionArgs& a, hipStream_t stream) {
     if (a.w.max_voxels <= kFewRows) {
         using F = AttentionShape<typename S::Type, S::kDim, 1, 1, S::KB>;
-        hipLaunchKernelGGL((voxel_attention_few<F, CAP, BIAS>), dim3((unsigned)(ceil_div(a.w.max_voxels, kFewPlaces) * a.heads)), dim3(kAttentionBlock), 0, stream, a);
+        const dim3 grid((unsigned)(ceil_div(a.w.max_voxels, kFewPlaces) * a.heads));
+        if (sizeof(typename S::Type) == 4 || a.w.max_voxels * a.heads <= kSharedRows) {
+            hipLaunchKernelGGL((voxel_attention_few<F, CAP, BIAS, true>), grid, dim3(kAttentionBlock), 0, stream, a);
+        } else if constexpr (sizeof(typename S::Type) == 2) {
+            hipLaunchKernelGGL((voxel_attention_few<F, CAP, BIAS, false>), grid, dim3(kAttentionBlock), 0, stream, a);
+        }
         return;
     }
     // (a tiny window's share of a workgroup is a quarter; what is beyond the grid is taken in turns)

@@ -269,6 +269,20 @@ def test_two_calls_at_once(rows):
             assert torch.equal(g, w)
 
 
+@pytest.mark.parametrize("dtype", [HALF, FLOAT])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(13, 13, 16), (24, 3, 32), (16, 16, 128), (2, 1, 128), (1, 1, 64)])
+@pytest.mark.parametrize("window", [(9, 40, 50), (9, 9, 9)])
+def test_few_rows_and_many_heads(dtype, heads, kv_heads, dim, window):
+    """Rows times heads either side of where a query's keys are shared out among the waves."""
+    rows = 2600
+    qkv, coors = make(rows, heads, kv_heads, dim, dtype)
+    case = Case(heads, kv_heads, dim, window, slopes=np.linspace(0, 1, heads))
+    op = case.op(rows)
+    got = op(dev(qkv), dev(coors), num(rows - 1))
+    case.check(got, qkv, coors, rows - 1)
+    assert torch.equal(op(dev(qkv), dev(coors), num(rows - 1)), got)
+
+
 def test_rows_beyond_32_bit_offsets():
     """qkv of more than 2^31 elements: the windows of the last rows."""
     rows, heads, dim = 360000, 16, 128
