@@ -210,6 +210,10 @@ struct AttentionShape {
     // Where the waves of a workgroup share the keys out: keys of a wave's block (up to eight words of a lane), its keys and values in LDS
     static constexpr int KW = 256 / kWordsHead > 64 ? 64 : 256 / kWordsHead < 16 ? 16 : 256 / kWordsHead;
     static constexpr int kWave = 2 * KW * Op::kPitch;
+    // Waves of a SIMD that the registers leave room for.  A third one is worth a few registers in memory: 30 000 keys, 8 heads of 64 values on 4 of keys
+    // 5.9 -> 5.4 ms, few rows 4 096 and 16 heads of 64 values in FP32 943 -> 830 us, 4 096 and 8 of 64 in FP16 194 -> 179.  Kernels that keep to 168
+    // by themselves are scheduled worse under the bound (53 000 rows, 8 heads of 32: 102 -> 106), those beyond 180 lose too many.
+    static constexpr int kWavesListed = DP == 64 && HG == 2 && KVG == 1 ? 3 : 2, kWavesFew = DP <= 64 ? 3 : 2;
 };
 
 enum { kCapNone, kCapExponential, kCapSeries };
@@ -598,7 +602,7 @@ __device__ __forceinline__ void shared_rows(const AttentionArgs& a, int start, i
 }
 
 template <typename S, int CAP, bool BIAS>
-__global__ void __launch_bounds__(kAttentionBlock, 2)
+__global__ void __launch_bounds__(kAttentionBlock, S::kWavesListed)
 voxel_attention(AttentionArgs a) {
     using T = typename S::Type;
     using Op = typename S::Op;
@@ -654,7 +658,7 @@ constexpr int kFewPlaces = 16;
 // 64 430 and 520, and windows of 60 rows at 4 096 rows and 16 heads 28 and 40.  FP32, whose products take longer: 4 096 rows and 16 heads of 64 1 509 and 936.
 constexpr int kSharedRows = 32768;  // rows times heads, FP16
 template <typename S, int CAP, bool BIAS, bool SHARED>
-__global__ void __launch_bounds__(kAttentionBlock, 2)
+__global__ void __launch_bounds__(kAttentionBlock, S::kWavesFew)
 voxel_attention_few(AttentionArgs a) {
     using T = typename S::Type;
     using Op = typename S::Op;
