@@ -413,12 +413,12 @@ typedef struct sessd_voxelattn_desc {
     int32_t spatial_shape[3]; /* x,y,z */
     int32_t window_shape[3];  /* x,y,z, cells; at most 2^22 windows in the grid */
     int32_t window_shift[3];  /* x,y,z, 0 .. window_shape - 1 */
-    float cell_size[3];       /* x,y,z: of a cell, in the unit that the slopes are per */
-    float softmax_scale;      /* 0 = 1 / sqrt(head_dim) */
-    float score_cap;          /* 0 = none */
+    float cell_size[3];       /* x,y,z: of a cell, in the unit that the slopes are per; at most 2^20 */
+    float softmax_scale;      /* 0 = 1 / sqrt(head_dim); of magnitude 2^-40 .. 2^40 */
+    float score_cap;          /* 0 = none; 2^-40 .. 2^40 */
 } sessd_voxelattn_desc;
 
-/* slopes: host FP32 [num_heads], finite, or NULL for no bias */
+/* slopes: host FP32 [num_heads], up to 2^20 of magnitude, or NULL for no bias */
 int sessd_voxelattn_create(const sessd_voxelattn_desc* desc, const float* slopes, sessd_voxelattn** out);
 int sessd_voxelattn_deserialize(const void* bytes, size_t n, sessd_voxelattn** out);
 size_t sessd_voxelattn_serialization_size(const sessd_voxelattn* h);

@@ -58,11 +58,17 @@ int VoxelAttentionPlugin::create(const sessd_voxelattn_desc& d, const float* slo
         return fail(SESSD_E_UNSUPPORTED, "voxelattn: %d x %d x %d windows, at most %d are supported", g.count[2], g.count[1], g.count[0], (int)kMostWindows);
     if (!std::isfinite(d.softmax_scale) || !std::isfinite(d.score_cap) || d.score_cap < 0.f)
         return fail(SESSD_E_INVALID, "voxelattn: softmax_scale and score_cap must be finite, score_cap not negative");
+    // (what a score is divided by and what a distance is times stays finite in FP32)
+    const float scale = std::fabs(d.softmax_scale), cells = std::fmax(std::fabs(d.cell_size[0]), std::fmax(std::fabs(d.cell_size[1]), std::fabs(d.cell_size[2])));
+    if ((scale != 0.f && (scale < 0x1p-40f || scale > 0x1p40f)) || (d.score_cap != 0.f && (d.score_cap < 0x1p-40f || d.score_cap > 0x1p40f)) || cells > 0x1p20f)
+        return fail(SESSD_E_UNSUPPORTED, "voxelattn: softmax_scale and score_cap must be 0 or 2^-40 .. 2^40, cell_size at most 2^20");
     std::unique_ptr<VoxelAttentionPlugin> p(new VoxelAttentionPlugin());
     p->desc_ = d;
     if (slopes) {
-        for (int h = 0; h < d.num_heads; ++h)
+        for (int h = 0; h < d.num_heads; ++h) {
             if (!std::isfinite(slopes[h])) return fail(SESSD_E_INVALID, "voxelattn: the slopes must be finite");
+            if (std::fabs(slopes[h]) > 0x1p20f) return fail(SESSD_E_UNSUPPORTED, "voxelattn: slopes beyond 2^20");
+        }
         p->slopes_.assign(slopes, slopes + d.num_heads);
         SESSD_HIP_TRY(hipMalloc(reinterpret_cast<void**>(&p->slopes_dev_), d.num_heads * sizeof(float)));
         SESSD_HIP_TRY(hipMemcpy(p->slopes_dev_, slopes, d.num_heads * sizeof(float), hipMemcpyHostToDevice));

@@ -455,11 +455,29 @@ class Sparse2Dense(_Plugin):
         return int(self.ws[:4].view(torch.int32)[0].item())
 
 
+def _current_device():
+    torch = _torch()
+    try:
+        return torch._C._cuda_getDevice()
+    except AttributeError:  # (a private name: a torch without it)
+        return torch.cuda.current_device()
+
+
 def _dense(*tensors):
-    """The library reads and writes rows one behind the other: views with other strides are refused."""
+    """The library reads and writes rows one behind the other, in memory of the current device: other tensors are refused."""
+    device = tensors[0].get_device()
     for t in tensors:
         if not t.is_contiguous():
             raise SessdError("a tensor is not contiguous: shape %s, strides %s" % (tuple(t.shape), t.stride()))
+        if t.get_device() != device or device < 0:
+            raise SessdError("a tensor is not in GPU memory, or not in that of the others: shape %s, %s" % (tuple(t.shape), t.device))
+    if device != _current_device():
+        raise SessdError("the tensors are on device %d, the current one is %d" % (device, _current_device()))
+
+
+def _windows_key(max_voxels, spatial_shape, window, shift):
+    """What two layers have alike that share their windows."""
+    return (int(max_voxels),) + tuple(tuple(int(v) for v in a) for a in (spatial_shape, window, shift))
 
 
 class RmsNorm(_Plugin):
@@ -535,6 +553,7 @@ class VoxelAttention(_Plugin):
         check(lib().sessd_voxelattn_create(C.byref(d), _np_f32_ptr(s), C.byref(h)))
         super().__init__(h)
         self.max_voxels, self.cout = max_voxels, num_heads * head_dim
+        self.windows = _windows_key(max_voxels, spatial_shape_xyz, window_xyz, shift_xyz)
 
     def __call__(self, qkv, coors, voxel_num, stream=None, windows_from=None):
         """qkv [max_voxels, (num_heads + 2 num_kv_heads) * head_dim] -> [max_voxels, num_heads * head_dim].  windows_from: a layer on
@@ -547,6 +566,9 @@ class VoxelAttention(_Plugin):
         if windows_from is None:
             self._enqueue_bound(bound, ins, outs, stream)
         else:
+            if windows_from.windows != self.windows or windows_from.ws is None:
+                raise SessdError("windows_from: a layer that has run on the same windows (max_voxels, grid, window, shift): %s, %s"
+                                 % (windows_from.windows, self.windows))
             check(lib().sessd_voxelattn_enqueue_shared(self.h, bound.ins, bound.outs, _pointers(ins), _pointers(outs),
                                                        _ptr(windows_from.ws), _stream_ptr(stream)))
         return out
@@ -595,6 +617,7 @@ def create_plugin(plugin_name, fields):
         obj.max_voxels, obj.cout = int(g("max_voxels")[0]), int(g("out_channel")[0])
     elif cls is VoxelAttention:
         obj.max_voxels, obj.cout = int(g("max_voxels")[0]), int(g("num_heads")[0]) * int(g("head_dim")[0])
+        obj.windows = _windows_key(obj.max_voxels, *(g(k) for k in ("spatial_shape", "window_shape", "window_shift")))
     else:
         obj.max_voxels, obj.cout = int(g("max_voxels")[0]), int(g("out_channel")[0])
         k = g("ksize")

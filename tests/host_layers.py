@@ -78,7 +78,8 @@ def check_create():
                      (dict(shift=(0, -1, 0)), E), (dict(grid=(70, 0, 10)), E), (dict(grid=(1 << 25, 1, 1), window=(1 << 20, 1, 1)), U),
                      (dict(grid=(4096, 1024, 2), window=(1, 1, 1)), U), (dict(grid=(1 << 24, 1 << 24, 1 << 24), window=(1, 1, 1)), U),
                      (dict(cell=(1, float("nan"), 1)), E), (dict(cap=-1.0), E), (dict(cap=float("inf")), E), (dict(scale=float("nan")), E),
-                     (dict(slopes=[0, 1, float("inf"), 2]), E)):
+                     (dict(slopes=[0, 1, float("inf"), 2]), E), (dict(scale=1e-13), U), (dict(scale=-2e12), U), (dict(cap=1e-20), U), (dict(cap=1e20), U),
+                     (dict(cell=(1, -3e6, 1)), U), (dict(slopes=[0, 1, 2, -2e6]), U)):
         refused(attention(**kw)[0], code, "voxelattn")
     assert attention(grid=(4096, 1024, 1), window=(1, 1, 1))[0] == 0       # 2^22 windows
     assert L.sessd_rmsnorm_create(None, None, None) == E and L.sessd_linear8_create(None, None, None) == E

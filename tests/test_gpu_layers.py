@@ -307,6 +307,8 @@ def test_wrong_tensors_are_refused():
     norm = api.RmsNorm(100, np.ones(100, np.float32), max_voxels=64)
     with pytest.raises(api.SessdError, match="contiguous"):
         norm(torch.randn(100, 64, device=DEV).half().t(), num(64))
+    with pytest.raises(api.SessdError, match="not in GPU memory"):
+        norm(f, num(64).cpu())
     with pytest.raises(api.SessdError, match="feat must be"):
         norm(f[:, :96].contiguous(), num(64))
     with pytest.raises(api.SessdError, match="feat must be"):

@@ -220,6 +220,21 @@ def test_the_same_bits_each_time_and_on_shared_windows(dtype, window, rows):
         assert torch.equal(got[:rows - 100][dev(keep)], a[:rows - 100][dev(keep)])
 
 
+def test_windows_of_another_kind_are_not_shared():
+    case = Case(2, 2, 16, (9, 6, 6))
+    qkv, coors = make(100, 2, 2, 16, HALF)
+    x, c, n = dev(qkv), dev(coors), num(100)
+    op = case.op(100)
+    for first, rows in ((Case(2, 2, 16, (9, 6, 6)), 90), (Case(2, 2, 16, (9, 6, 7)), 100), (Case(2, 2, 16, (9, 6, 6), shift=(0, 1, 0)), 100),
+                        (Case(2, 2, 16, (9, 6, 6), grid=(9, 40, 51)), 100)):
+        other = first.op(rows)
+        other(x[:rows], c[:rows], n)
+        with pytest.raises(api.SessdError, match="windows_from"):
+            op(x, c, n, windows_from=other)
+    with pytest.raises(api.SessdError, match="windows_from"):  # (has not run)
+        op(x, c, n, windows_from=case.op(100))
+
+
 def test_order_of_rows_does_not_choose_neighbours():
     """The same voxels in another order: the same outputs up to the order of their sums."""
     case = Case(2, 2, 16, (9, 6, 6), slopes=[1, 2])

@@ -47,3 +47,12 @@ def test_struct_layouts_match_the_header(tmp_path):
         assert int(out[cname]) == C.sizeof(mirror)
         for f, _ in mirror._fields_:
             assert int(out["%s.%s" % (cname, f)]) == getattr(mirror, f).offset
+
+
+def test_tensors_in_host_memory_are_refused():
+    import torch
+    from sessd3d import api
+    with pytest.raises(api.SessdError, match="not in GPU memory"):
+        api._dense(torch.zeros(4, 4))
+    with pytest.raises(api.SessdError, match="contiguous"):
+        api._dense(torch.zeros(4, 6).t())
