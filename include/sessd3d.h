@@ -430,7 +430,8 @@ int sessd_voxelattn_enqueue(sessd_voxelattn* h, const sessd_tensor_desc* inDesc,
                             const void* const* inputs, void* const* outputs, void* workspace, sessd_stream_t stream);
 /* The layer on the windows that an earlier sessd_voxelattn_enqueue left in `window_workspace` (same coors, voxel_num,
  * max_voxels, spatial_shape, window_shape and window_shift; heads, slopes and the rest may differ): consecutive layers on
- * one coors tensor find their windows once.  The same bits as sessd_voxelattn_enqueue. */
+ * one coors tensor find their windows once.  The same bits as sessd_voxelattn_enqueue.  The rows that there are, are those of
+ * the earlier call, whatever coors and voxel_num hold by now. */
 int sessd_voxelattn_enqueue_shared(sessd_voxelattn* h, const sessd_tensor_desc* inDesc, const sessd_tensor_desc* outDesc,
                                    const void* const* inputs, void* const* outputs, const void* window_workspace,
                                    sessd_stream_t stream);

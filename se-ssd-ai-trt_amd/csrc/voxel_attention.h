@@ -24,7 +24,6 @@ namespace sessd {
 struct AttentionArgs {
     const void* qkv;
     void* out;
-    const int32_t* voxel_num;
     const float* slopes;  // or null
     WindowIndex w;
     int heads, kv_heads, dim;
@@ -645,7 +644,7 @@ voxel_attention(AttentionArgs a) {
         }
     }
     // rows that attend to nothing: outside the grid, and behind the last one
-    const int n = clamp_rows(a.voxel_num, a.w.max_voxels), places = a.w.head[kHeadPlaces];
+    const int n = a.w.head[kHeadRows], places = a.w.head[kHeadPlaces];
     const size_t row_words = (size_t)a.heads * a.dim / Op::kPer;
     const size_t thread = (size_t)blockIdx.x * kAttentionBlock + tid, threads = (size_t)gridDim.x * kAttentionBlock;
     for (size_t i = thread; i < (size_t)(n - places) * row_words; i += threads)
@@ -673,7 +672,7 @@ voxel_attention_few(AttentionArgs a) {
     T* const out = static_cast<T*>(a.out);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int first = (int)(blockIdx.x / (unsigned)a.heads) * kFewPlaces, head = (int)(blockIdx.x % (unsigned)a.heads);
-    const int n = clamp_rows(a.voxel_num, a.w.max_voxels), places = a.w.head[kHeadPlaces];
+    const int n = a.w.head[kHeadRows], places = a.w.head[kHeadPlaces];
     const int place = first + lane;
     const bool there = lane < kFewPlaces && place < places;
     const int2 span = there ? a.w.span[place] : make_int2(0, 0);  // (every wave has all of them)

@@ -140,7 +140,6 @@ int VoxelAttentionPlugin::attend(const void* const* inputs, void* const* outputs
     AttentionArgs a;
     a.qkv = inputs[0];
     a.out = outputs[0];
-    a.voxel_num = static_cast<const int32_t*>(inputs[2]);
     a.slopes = slopes_dev_;
     a.w = carve_windows(const_cast<void*>(workspace), desc_.max_voxels, grid_of(desc_).windows());
     a.heads = desc_.num_heads;

@@ -19,8 +19,9 @@ constexpr int kItemRows = 64;  // queries of a work item
 // Rows of a window: up to kTinyRows it is listed as a whole, beyond it has items, beyond kShortRows they are the long ones
 constexpr int kTinyRows = 32, kShortRows = 128;
 
-// Words of WindowIndex::head.  Four ranges that window_base takes stand one after the other
-enum { kHeadStatus = 0, kHeadPlaces, kHeadLong, kHeadShort, kHeadTiny, kHeadOutside, kHeadWords = 64 };
+// Words of WindowIndex::head.  Four ranges that window_base takes stand one after the other;
+// kHeadRows: voxel_num as the list was made, which later readers go by (rows that it does not name have no places)
+enum { kHeadStatus = 0, kHeadPlaces, kHeadLong, kHeadShort, kHeadTiny, kHeadOutside, kHeadRows, kHeadWords = 64 };
 
 // What a layer's workspace holds.  The list comes first: its place follows from max_voxels and the number of windows alone, which layers
 // on the same windows share.

@@ -43,8 +43,8 @@ window_count(const int32_t* __restrict__ coors, const int32_t* __restrict__ voxe
     int4 c = make_int4(-1, 0, 0, 0);
     if (row < w.max_voxels) c = reinterpret_cast<const int4*>(coors)[row];
     for (int i = threadIdx.x; i < windows / 8; i += kChunk) s_count4[i] = make_uint4(0, 0, 0, 0);
-    if (blockIdx.x == 0 && threadIdx.x < kHeadWords) w.head[threadIdx.x] = 0;
     const int n = clamp_rows(voxel_num, w.max_voxels);
+    if (blockIdx.x == 0 && threadIdx.x < kHeadWords) w.head[threadIdx.x] = threadIdx.x == kHeadRows ? n : 0;
     if ((int)blockIdx.x * kChunk >= n) return;
     const int key = row < n ? window_of(c, g) : -1;
     uint64_t same = __ballot(key >= 0);
@@ -173,6 +173,7 @@ window_few(const int32_t* __restrict__ coors, const int32_t* __restrict__ voxel_
     if (blockIdx.x == 0 && tid == 0) {
         w.head[kHeadStatus] = s_outside ? SESSD_STATUS_BAD_COORD : 0;
         w.head[kHeadPlaces] = n - s_outside;
+        w.head[kHeadRows] = n;
     }
     if ((int)blockIdx.x * kFewOwn >= n) return;
     // (the rows between n and end are behind all others: smaller than none, equal to those outside, in front of none)
@@ -211,6 +212,7 @@ __global__ void __launch_bounds__(kBlock)
 window_ticket(const int32_t* __restrict__ coors, const int32_t* __restrict__ voxel_num, WindowGrid g, WindowIndex w) {
     const int row = blockIdx.x * kBlock + threadIdx.x;
     const int n = clamp_rows(voxel_num, w.max_voxels);
+    if (row == 0) w.head[kHeadRows] = n;
     if (row >= n) return;
     const int key = window_of(reinterpret_cast<const int4*>(coors)[row], g);
     if (key < 0) set_outside(w, n, row);

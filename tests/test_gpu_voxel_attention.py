@@ -220,6 +220,23 @@ def test_the_same_bits_each_time_and_on_shared_windows(dtype, window, rows):
         assert torch.equal(got[:rows - 100][dev(keep)], a[:rows - 100][dev(keep)])
 
 
+@pytest.mark.parametrize("rows,window", [(900, (9, 6, 6)), (MANY, (9, 6, 6)), (MANY, (1, 1, 1))])
+def test_shared_windows_go_by_the_rows_they_were_found_for(rows, window):
+    """voxel_num and coors that another frame has overwritten by the time of the sharer's call."""
+    case = Case(2, 2, 16, window, grid=(9, 80, 80))  # (57 600 windows of one cell: by tickets)
+    qkv, coors = make(rows, 2, 2, 16, HALF, grid=(9, 80, 80))
+    coors[7, 1] = 9  # outside
+    first, second = case.op(rows), case.op(rows)
+    for m in (500, 0):
+        c, n = dev(coors), num(m)
+        a = first(dev(qkv), c, n)
+        case.check(a, qkv, coors, m)
+        for other in (rows, 3, -5):
+            n.fill_(other)
+            c.fill_(-1 if other == 3 else 2)
+            assert torch.equal(second(dev(qkv), c, n, windows_from=first), a)
+
+
 def test_windows_of_another_kind_are_not_shared():
     case = Case(2, 2, 16, (9, 6, 6))
     qkv, coors = make(100, 2, 2, 16, HALF)
