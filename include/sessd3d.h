@@ -385,7 +385,8 @@ size_t sessd_linear8_workspace_size(const sessd_linear8* h, const sessd_tensor_d
                                     const sessd_tensor_desc* out, int nOut);
 int sessd_linear8_enqueue(sessd_linear8* h, const sessd_tensor_desc* inDesc, const sessd_tensor_desc* outDesc,
                           const void* const* inputs, void* const* outputs, void* workspace, sessd_stream_t stream);
-/* As sessd_submconv3d_set_epilogue. */
+/* As sessd_submconv3d_set_epilogue.  Waits for all that the device has queued: earlier calls have the old epilogue on any stream, later ones the
+ * new one, and so do replays of calls that a graph has captured before.  What fails changes nothing. */
 int sessd_linear8_set_epilogue(sessd_linear8* h, const float* scale, const float* shift, int relu);
 int sessd_linear8_set_flags(sessd_linear8* h, int32_t flags);
 void sessd_linear8_destroy(sessd_linear8* h);

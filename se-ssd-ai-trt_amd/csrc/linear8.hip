@@ -15,6 +15,7 @@
 // 760 TFLOP/s; 60 000 rows 512 -> 128 FP32 21 us; weights read anew for every 16 rows 359 and 44 us.  Inputs beyond kMostHeld, whose weights no
 // wave's registers hold, do read them anew.
 #include <cmath>
+#include <utility>
 
 #include "plugins.h"
 
@@ -51,9 +52,9 @@ struct LinearArgs {
     const uint8_t* q;
     const float* scale;
     const int32_t* voxel_num;
-    int max_voxels, cin, cout, relu, write_pad;
+    int max_voxels, cin, cout, write_pad;
     const __half* w;       // [block of columns][step][instruction][lane][8]
-    const float* columns;  // of the result: factor, addend; two rows of whole blocks
+    const float* columns;  // of the result: factor, addend, two rows of whole blocks; behind them 1 for a ReLU
     void* out;
 };
 
@@ -65,7 +66,7 @@ __device__ __forceinline__ void put(V* to, const V& x) {
 
 // A lane's 4 NT columns of a row, of the block of columns from `c0` on
 template <typename T, int NT>
-__device__ __forceinline__ void store_columns(const LinearArgs& a, int row, int c0, const v4f (&acc)[NT], float s, const float* factor, const float* addend, int g) {
+__device__ __forceinline__ void store_columns(const LinearArgs& a, int row, int c0, const v4f (&acc)[NT], float s, const float* factor, const float* addend, bool relu, int g) {
     constexpr bool kHalf = sizeof(T) == 2;
     T* const dst = static_cast<T*>(a.out) + (size_t)row * a.cout + c0;
     const bool whole = a.cout % (16 / (int)sizeof(T)) == 0 && c0 + 16 * NT <= a.cout;
@@ -77,7 +78,7 @@ __device__ __forceinline__ void store_columns(const LinearArgs& a, int row, int 
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[t][e] = fmaf(acc[t][e] * s, f[e], b[e]);
     }
-    if (a.relu) {
+    if (relu) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -128,6 +129,7 @@ linear8_held(LinearArgs a) {
     if (lane < kWide)
 #pragma unroll
         for (int i = 0; i < 2; ++i) s_columns[wave][i][lane] = a.columns[i * blocks * kWide + cb * kWide + lane];
+    const bool relu = a.columns[2 * blocks * kWide] != 0.f;
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -168,7 +170,7 @@ linear8_held(LinearArgs a) {
         for (int k = 0; k < 2 * PAIRS; ++k)
 #pragma unroll
             for (int t = 0; t < NT; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[k][t], b[k], acc[t], 0, 0, 0);
-        if (first + r < rows) store_columns<T, NT>(a, first + r, cb * kWide, acc, s, s_columns[wave][0], s_columns[wave][1], g);
+        if (first + r < rows) store_columns<T, NT>(a, first + r, cb * kWide, acc, s, s_columns[wave][0], s_columns[wave][1], relu, g);
     }
 }
 
@@ -192,7 +194,7 @@ linear8_wide(LinearArgs a) {
         }
     }
     if (row >= a.max_voxels || (row >= n && !a.write_pad)) return;
-    store_columns<T, NT>(a, row, cb * kWide, acc, row < n ? a.scale[row] : 0.f, a.columns + cb * kWide, a.columns + (blocks + cb) * kWide, g);
+    store_columns<T, NT>(a, row, cb * kWide, acc, row < n ? a.scale[row] : 0.f, a.columns + cb * kWide, a.columns + (blocks + cb) * kWide, a.columns[2 * blocks * kWide] != 0.f, g);
 }
 
 template <typename T>
@@ -274,20 +276,29 @@ int Linear8Plugin::create(const sessd_linear8_desc& d, const float* weights, Lin
         SESSD_HIP_TRY(hipMemcpy(p->weights_packed_dev_ + (half ? count : 0), packed.data(), count * sizeof(uint16_t), hipMemcpyHostToDevice));
     }
     p->packed_count_ = count;
-    SESSD_TRY(p->uploadColumns());
+    SESSD_TRY(p->uploadColumns(p->epi_));
     *out = p.release();
     return SESSD_OK;
 }
 
-// factor and addend of a column, for whole blocks of columns
-int Linear8Plugin::uploadColumns() {
+// Factor and addend of a column, for whole blocks of columns, and whether there is a ReLU.  All of it is in device memory, at an address that stays:
+// calls in a captured graph have the new epilogue as a whole from their next replay on.  Queued calls on any stream may still read the old one.
+// hipMemcpy waits for the default stream alone, hipFree for all that the device has.
+int Linear8Plugin::uploadColumns(const Epilogue& e) {
     const size_t pad = (size_t)padded_columns(in_channel_, out_channel_);
-    std::vector<float> host(2 * pad, 0.f);
+    std::vector<float> host(2 * pad + 1, 0.f);
     for (int c = 0; c < out_channel_; ++c) {
-        host[c] = epi_.scale_host.empty() ? wscale_[c] : wscale_[c] * epi_.scale_host[c];
-        host[pad + c] = epi_.shift_host.empty() ? 0.f : epi_.shift_host[c];
+        host[c] = e.scale_host.empty() ? wscale_[c] : wscale_[c] * e.scale_host[c];
+        host[pad + c] = e.shift_host.empty() ? 0.f : e.shift_host[c];
     }
-    if (!columns_dev_) SESSD_HIP_TRY(hipMalloc(reinterpret_cast<void**>(&columns_dev_), host.size() * sizeof(float)));
+    host[2 * pad] = e.relu ? 1.f : 0.f;
+    if (columns_dev_) {
+        void* wait = nullptr;
+        SESSD_HIP_TRY(hipMalloc(&wait, 256));
+        SESSD_HIP_TRY(hipFree(wait));
+    } else {
+        SESSD_HIP_TRY(hipMalloc(reinterpret_cast<void**>(&columns_dev_), host.size() * sizeof(float)));
+    }
     SESSD_HIP_TRY(hipMemcpy(columns_dev_, host.data(), host.size() * sizeof(float), hipMemcpyHostToDevice));
     return SESSD_OK;
 }
@@ -297,8 +308,9 @@ int Linear8Plugin::setEpilogue(const float* scale, const float* shift, int relu)
     e.relu = relu ? 1 : 0;
     if (scale) e.scale_host.assign(scale, scale + out_channel_);
     if (shift) e.shift_host.assign(shift, shift + out_channel_);
-    epi_ = e;
-    return uploadColumns();
+    SESSD_TRY(uploadColumns(e));
+    epi_ = std::move(e);
+    return SESSD_OK;
 }
 
 // in_channel, out_channel, max_voxels, weights, the epilogue as the convolutions write it
@@ -375,7 +387,6 @@ int Linear8Plugin::enqueue(const sessd_tensor_desc* inputDesc, const sessd_tenso
     a.max_voxels = max_voxels_;
     a.cin = in_channel_;
     a.cout = out_channel_;
-    a.relu = epi_.relu;
     a.write_pad = (flags_ & SESSD_FLAG_SKIP_PAD_ROWS) ? 0 : 1;
     a.w = weights_packed_dev_ + (out_type_ == SESSD_HALF ? packed_count_ : 0);
     a.columns = columns_dev_;

@@ -320,14 +320,14 @@ class Linear8Plugin {
     std::vector<float> weights_;         // as given, FP32 [Cin][Cout]
     __half* weights_packed_dev_ = nullptr;  // e4m3 values as halves, operand order (linear8.hip): for FP32 outputs, for FP16 ones
     size_t packed_count_ = 0;            // of either
-    float* columns_dev_ = nullptr;       // factor and addend of each column (linear8.hip)
+    float* columns_dev_ = nullptr;       // the epilogue: factor and addend of each column (linear8.hip)
     Epilogue epi_;                       // (host side; the device has it in columns_dev_)
     int out_type_ = SESSD_FLOAT;
     int flags_ = 0;
 
   private:
     int check(const sessd_tensor_desc* in, const sessd_tensor_desc* out) const;
-    int uploadColumns();
+    int uploadColumns(const Epilogue& e);
     std::vector<float> wscale_;
 };
 

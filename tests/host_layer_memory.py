@@ -1,0 +1,99 @@
+"""What RmsNorm, Linear8 and VoxelAttention keep in device memory, on the stand-in runtime of fake_hip_memory.cpp, without torch and without a GPU: run
+as a program of its own (tests/test_layer_memory_cpu.py), because one process holds one HIP runtime.
+
+    python tests/host_layer_memory.py <path of the stand-in library> <check>
+"""
+import ctypes as C
+import os
+import sys
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path[:0] = [os.path.join(ROOT, "se-ssd-ai-trt_amd"), os.path.join(ROOT, "tests")]
+sys.modules["torch"] = None  # (sessd3d.api binds the library to torch's runtime where it finds torch)
+
+import numpy as np  # noqa: E402
+from sessd3d import api, ctypes_defs as D  # noqa: E402
+
+FAKE = C.CDLL(sys.argv[1], mode=C.RTLD_GLOBAL)
+FAKE.fake_log.restype = C.c_char_p
+FAKE.fake_largest_allocation.argtypes = [C.c_ulonglong]
+FAKE.fake_fail_copy.argtypes = [C.c_long]
+L = api.lib()
+I32, F32, F16, FP8 = D.SESSD_INT32, D.SESSD_FLOAT, D.SESSD_HALF, D.SESSD_FP8
+
+
+def log():
+    lines = [l.split() for l in FAKE.fake_log().decode().splitlines()]
+    FAKE.fake_clear_log()
+    return lines
+
+
+def of_kind(lines, kind):
+    return [(int(a), int(b)) for k, a, b in lines if k == kind]
+
+
+def descs(*shapes):
+    return (D.TensorDesc * len(shapes))(*[D.TensorDesc.make(list(s), t) for s, t in shapes])
+
+
+def pointers(*values):
+    return (C.c_void_p * len(values))(*values)
+
+
+class Linear:
+    def __init__(self, cin, cout, w, rows=100):
+        log()
+        self.h = C.c_void_p()
+        w = np.ascontiguousarray(w, np.float32)
+        assert L.sessd_linear8_create(C.byref(D.Linear8Desc(cin, cout, rows)), w.ctypes.data, C.byref(self.h)) == 0
+        self.memory = of_kind(log(), "malloc")
+        self.ins = descs(((1, rows, cin), FP8), ((1, rows, 1), F32), ((1,), I32))
+        self.cout, self.rows = cout, rows
+
+    def call(self, dtype=F16):
+        outs = descs(((1, self.rows, self.cout), dtype))
+        assert L.sessd_linear8_configure(self.h, self.ins, 3, outs, 1) == 0
+        return L.sessd_linear8_enqueue(self.h, self.ins, outs, pointers(4096, 8192, 64), pointers(16384), None, None)
+
+    def set_epilogue(self, scale, shift, relu):
+        p = lambda a: None if a is None else np.ascontiguousarray(a, np.float32).ctypes.data_as(C.c_void_p)  # noqa: E731
+        return L.sessd_linear8_set_epilogue(self.h, p(scale), p(shift), relu)
+
+    def blob(self):
+        buf = C.create_string_buffer(L.sessd_linear8_serialization_size(self.h))
+        assert L.sessd_linear8_serialize(self.h, buf) == 0
+        return buf.raw
+
+    def device_memory(self):
+        return [C.string_at(p, n) for p, n in self.memory]
+
+
+def check_epilogue():
+    """A new epilogue waits for the calls that read the old one, and one that cannot be had changes nothing."""
+    rng = np.random.default_rng(0)
+    lin = Linear(32, 20, rng.standard_normal((32, 20)))
+    sc, sh = rng.standard_normal((2, 20)).astype(np.float32)
+    assert lin.set_epilogue(sc, sh, 1) == 0
+    assert lin.call() == 0
+    log()
+    assert lin.set_epilogue(-sc, None, 0) == 0
+    assert not of_kind(log(), "unordered")
+    assert lin.call() == 0 and lin.set_epilogue(None, sh, 1) == 0 and not of_kind(log(), "unordered")
+    # what fails leaves the plugin and the GPU as they were
+    blob, memory = lin.blob(), lin.device_memory()
+    FAKE.fake_fail_copy(0)
+    assert lin.set_epilogue(sc, sh, 0) == D.SESSD_E_HIP
+    FAKE.fake_fail_copy(-1)
+    assert lin.blob() == blob and lin.device_memory() == memory
+    FAKE.fake_largest_allocation(16)
+    assert lin.set_epilogue(sc, sh, 0) == D.SESSD_E_HIP
+    FAKE.fake_largest_allocation(1 << 62)
+    assert lin.blob() == blob and lin.device_memory() == memory
+    L.sessd_linear8_destroy(lin.h)
+
+
+CHECKS = {k[6:]: v for k, v in list(globals().items()) if k.startswith("check_")}
+
+if __name__ == "__main__":
+    CHECKS[sys.argv[2]]()
+    print("ok")
