@@ -49,7 +49,7 @@ int VoxelAttentionPlugin::create(const sessd_voxelattn_desc& d, const float* slo
     for (int a = 0; a < 3; ++a) {
         if (d.spatial_shape[a] < 1 || d.window_shape[a] < 1 || d.window_shift[a] < 0 || d.window_shift[a] >= d.window_shape[a])
             return fail(SESSD_E_INVALID, "voxelattn: shapes must be positive, shifts 0 .. window_shape - 1");
-        if (d.spatial_shape[a] > 1 << 24 || d.window_shape[a] > 1 << 24)  // (a cell's place is exact in FP32)
+        if (d.spatial_shape[a] > 1 << 24 || d.window_shape[a] > 1 << 24)  // (a cell, and the difference of two, is exact in FP32)
             return fail(SESSD_E_UNSUPPORTED, "voxelattn: shapes beyond 2^24 cells");
         if (!std::isfinite(d.cell_size[a])) return fail(SESSD_E_INVALID, "voxelattn: cell_size must be finite");
     }

@@ -1,0 +1,53 @@
+"""VoxelAttention on the GPU where FP32 and FP16 run out of bits: against 64 bits, with bounds from the formula alone (attention_bounds.py)."""
+import numpy as np
+import pytest
+import torch
+
+import attention_bounds as A
+from gpu_util import dev
+from sessd3d import api
+
+pytestmark = pytest.mark.gpu
+HALF, FLOAT = torch.float16, torch.float32
+# Rows of the tensor that holds a window: a few, those whose windows are listed, and so many that a workgroup takes two heads in FP16
+CAPACITIES = [None, 6000, 100500]
+
+
+def num(n):
+    return dev(np.array([n], np.int32))
+
+
+def attend(qkv, cells, grid_zyx, heads, kv_heads, dim, capacity=None, **kw):
+    """One window as large as the grid; the tensor's rows behind the window's are NaN."""
+    n = len(qkv)
+    rows = max(n, capacity or n)
+    x = np.full((rows, qkv.shape[1]), np.nan, qkv.dtype)
+    coors = np.full((rows, 4), -1, np.int32)
+    x[:n], coors[:n, 0], coors[:n, 1:] = qkv, 0, cells
+    op = api.VoxelAttention(heads, kv_heads, dim, grid_zyx[::-1], grid_zyx[::-1], max_voxels=rows, **kw)
+    got = op(dev(x), dev(coors), num(n))
+    assert op.status() == 0
+    return got.cpu().numpy()[:n].astype(np.float64)
+
+
+def assert_within(got, want, tol):
+    off = ~(np.abs(got - want) <= tol)
+    assert not off.any(), (int(off.sum()), float(np.nanmax(np.abs(got - want))), float((np.abs(got - want) / tol)[off].max()))
+
+
+@pytest.mark.parametrize("capacity", CAPACITIES)
+@pytest.mark.parametrize("dtype", [HALF, FLOAT])
+@pytest.mark.parametrize("length,cell,slope", [(1600, 0.05, 40.0), (100000, 0.05, 20.0), (1 << 24, 0.3, 4.0), (1 << 24, 1e-3, 1e3)])
+def test_distances_far_from_the_windows_first_cell(dtype, length, cell, slope, capacity):
+    """Neighbours at the far end of a long window: their distance has the bits that it has anywhere else."""
+    rng = np.random.default_rng(length)
+    n, heads, dim = 300, 2, 16
+    cells = np.zeros((n, 3), np.int64)
+    cells[:, 2] = length - 1 - rng.choice(min(length, 900), n, replace=False)
+    cells[:, 1] = rng.integers(0, 40, n)
+    cells[:, 0] = rng.integers(0, 4, n)
+    qkv = rng.standard_normal((n, 3 * heads * dim)).astype(np.float16 if dtype == HALF else np.float32)
+    size = (2 * cell, cell, cell)  # z,y,x
+    slopes = np.array([slope, slope / 7], np.float32)
+    want, tol = A.one_window(qkv, cells, heads, heads, dim, slopes, size, scale=0.25)
+    assert_within(attend(qkv, cells, (4, 40, length), heads, heads, dim, capacity, slopes=slopes, cell_size_xyz=size[::-1]), want, tol)
