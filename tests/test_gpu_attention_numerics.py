@@ -51,3 +51,40 @@ def test_distances_far_from_the_windows_first_cell(dtype, length, cell, slope, c
     slopes = np.array([slope, slope / 7], np.float32)
     want, tol = A.one_window(qkv, cells, heads, heads, dim, slopes, size, scale=0.25)
     assert_within(attend(qkv, cells, (4, 40, length), heads, heads, dim, capacity, slopes=slopes, cell_size_xyz=size[::-1]), want, tol)
+
+
+@pytest.mark.parametrize("capacity", CAPACITIES)
+@pytest.mark.parametrize("dtype,exponent", [(t, e) for t in (HALF, FLOAT) for e in (20, 26, 29, 32, 35)] + [(FLOAT, 60)])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("n", [20, 60, 700])
+def test_scores_of_any_size(dtype, exponent, bias, n, capacity):
+    """Scores of some 2^exponent, apart by at least a thousandth of that: the largest one's key takes all, and scores that are the same share."""
+    rng = np.random.default_rng(exponent)
+    heads, dim, t = 2, 64, np.float16 if dtype == HALF else np.float32
+    cells = np.stack(np.unravel_index(np.arange(n), (1, 28, 25)), 1)
+    qkv = np.zeros((n, 3 * heads * dim), t)
+    each = 2.0 ** ((exponent - 6) / 2)  # of 64 products, that of a query's value and a key's
+    for h in range(heads):
+        key = np.rint(rng.permutation(n) * (1000.0 / n)) + 1000.0   # (1000 .. 2000, of 11 bits: what they are times is a power of two)
+        key[rng.integers(n, size=n // 4)] = key.max()
+        sign = rng.choice([-1.0, 1.0], n)
+        qkv[:, h * dim:(h + 1) * dim] = (sign * 2.0 ** np.floor(np.log2(each)))[:, None]
+        qkv[:, (heads + h) * dim:(heads + h + 1) * dim] = (key * 2.0 ** (np.ceil(np.log2(each)) - 10))[:, None]
+    qkv[:, 2 * heads * dim:] = rng.standard_normal((n, heads * dim))
+    assert np.isfinite(qkv).all()
+    slopes = [0.5, 0.25] if bias else None
+    x = qkv.astype(np.float64)
+    want = np.zeros((n, heads * dim))
+    for h in range(heads):
+        q, k, v = (x[:, i * dim:(i + 1) * dim] for i in (h, heads + h, 2 * heads + h))
+        s = q @ k.T
+        if bias:  # (in FP32 it is less than a step of the score, or decides between scores that are the same)
+            far = np.sqrt(((cells[:, None] - cells[None]) ** 2).sum(2))
+            s = (s.astype(np.float32) - np.float32(slopes[h]) * far.astype(np.float32)).astype(np.float64)
+        p = np.exp(s - s.max(1, keepdims=True))
+        want[:, h * dim:(h + 1) * dim] = (p @ v) / p.sum(1, keepdims=True)
+    got = attend(qkv, cells, (1, 28, 25), heads, heads, dim, capacity, softmax_scale=1.0, slopes=slopes)
+    assert np.isfinite(got).all()
+    if not bias:  # equal weights of 1 or 2^14, and zeros
+        tol = (2.0 ** -11 if dtype == HALF else 8 * A.U) * np.abs(x[:, 2 * heads * dim:]).max() + n * A.U
+        assert_within(got, want, np.full(want.shape, tol))
