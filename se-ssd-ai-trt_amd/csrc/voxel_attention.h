@@ -101,6 +101,9 @@ template <int DP> struct Operand<_Float16, DP> {
         for (int s = 0; s < kParts; ++s) acc = product(k.part[s], q.part[s], acc);
         return acc;
     }
+    // A weight is held times 2^14.  The largest one of a row is that, and what is below FP16's steps is below 2^-39 of it: times 1, thousands of keys
+    // of 2^-25 would come to nothing, or to twice what they are.  (The factor is an addend that the exponent's fma has room for, and drops out with the sum.)
+    static constexpr float kLargest = 14.f;
     // The weights of 16 H keys, rounded to 11 bits: the product's own operands are FP16.  Their sum is taken by a product with ones, of the
     // weights as they are rounded.
     template <int H> struct Weights {
@@ -142,6 +145,7 @@ template <int DP> struct Operand<_Float16, DP> {
 
 template <int DP> struct Operand<float, DP> {
     static constexpr int kPer = 4, kPitch = DP + 4, kParts = DP / 16;
+    static constexpr float kLargest = 0.f;
     // 16x16x4: the j-th instruction of a part takes value 16 s + 4 (lane / 16) + j
     struct Row {
         v4f part[kParts];
@@ -274,7 +278,7 @@ __device__ __forceinline__ void attend(const AttentionArgs& a, v4f (&z)[H], cons
 #pragma unroll
     for (int t = 0; t < H; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) z[t][e] = __builtin_amdgcn_exp2f((z[t][e] - top) * a.by);
+        for (int e = 0; e < 4; ++e) z[t][e] = __builtin_amdgcn_exp2f(fmaf(z[t][e] - top, a.by, Op::kLargest));
     const typename Op::template Weights<H> p(z);
     total = Op::template add<H>(total, p);
 #pragma unroll

@@ -7,8 +7,9 @@ import numpy as np
 U = 2.0 ** -24
 
 
-def one_window(qkv, cells, heads, kv_heads, dim, slopes=None, cell=(1.0, 1.0, 1.0), cap=0.0, scale=1.0):
-    """qkv [rows, (heads + 2 kv_heads) dim], cells [rows, 3] integers -> output [rows, heads * dim], bound of the same shape.
+def one_window(qkv, cells, heads, kv_heads, dim, slopes=None, cell=(1.0, 1.0, 1.0), cap=0.0, scale=1.0, queries=None):
+    """qkv [rows, (heads + 2 kv_heads) dim], cells [rows, 3] integers -> output [rows, heads * dim], bound of the same shape;  of `queries` alone, if
+    there are any.
 
     A score t = scale q.k: within (dim + 2) u scale sum|q_d k_d| of itself; the cap, whose slope is at most 1, adds 8 u cap.  The difference
     of two cells is an integer below 2^24, exact in FP32; times the cells' size (u), squared (doubles that) with three products and
@@ -20,12 +21,15 @@ def one_window(qkv, cells, heads, kv_heads, dim, slopes=None, cell=(1.0, 1.0, 1.
     half = qkv.dtype == np.float16
     x = qkv.astype(np.float64)
     rows = len(x)
-    out, bound = np.zeros((rows, heads * dim)), np.zeros((rows, heads * dim))
-    diff = (cells[:, None].astype(np.int64) - cells[None].astype(np.int64)) * np.asarray(cell, np.float32).astype(np.float64)
-    far = np.sqrt((diff ** 2).sum(2))
+    of = np.arange(rows) if queries is None else np.asarray(queries)
+    out, bound = np.zeros((len(of), heads * dim)), np.zeros((len(of), heads * dim))
+    if slopes is not None:
+        diff = (cells[of][:, None].astype(np.int64) - cells[None].astype(np.int64)) * np.asarray(cell, np.float32).astype(np.float64)
+        far = np.sqrt((diff ** 2).sum(2))
     for h in range(heads):
         g = h // (heads // kv_heads)
         q, k, v = (x[:, i * dim:(i + 1) * dim] for i in (h, heads + g, heads + kv_heads + g))
+        q = q[of]
         t = scale * (q @ k.T)
         e = (dim + 2) * U * abs(scale) * (np.abs(q) @ np.abs(k).T)
         if cap:

@@ -88,3 +88,21 @@ def test_scores_of_any_size(dtype, exponent, bias, n, capacity):
     if not bias:  # equal weights of 1 or 2^14, and zeros
         tol = (2.0 ** -11 if dtype == HALF else 8 * A.U) * np.abs(x[:, 2 * heads * dim:]).max() + n * A.U
         assert_within(got, want, np.full(want.shape, tol))
+
+
+@pytest.mark.parametrize("capacity", CAPACITIES)
+@pytest.mark.parametrize("dtype", [HALF, FLOAT])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 1, 16), (2, 2, 32), (2, 1, 64)])
+@pytest.mark.parametrize("below", [9.0, 16.0, 17.25, 17.5, 20.0])
+def test_what_many_small_weights_add_up_to(dtype, heads, kv_heads, dim, below, capacity):
+    """One key takes nearly all, and thousands are `below` less than it, each of them below FP16's steps next to 1."""
+    n = 4000
+    cells = np.stack(np.unravel_index(np.arange(n), (4, 25, 40)), 1)
+    qkv = np.zeros((n, (heads + 2 * kv_heads) * dim), np.float16 if dtype == HALF else np.float32)
+    qkv[:, :heads * dim:dim] = 1.0
+    qkv[77, heads * dim:(heads + kv_heads) * dim:dim] = below
+    qkv[:, (heads + kv_heads) * dim:] = np.random.default_rng(0).uniform(0.5, 1.5, (n, kv_heads * dim))
+    qkv[77, (heads + kv_heads) * dim:] = 0.0
+    want, tol = A.one_window(qkv, cells, heads, kv_heads, dim, queries=[0])  # (all queries are the same)
+    assert (tol <= want * 0.01 + 2.0 ** -24).all()
+    assert_within(attend(qkv, cells, (4, 25, 40), heads, kv_heads, dim, capacity, softmax_scale=1.0), want, tol)
