@@ -437,6 +437,7 @@ int sessd_voxelattn_enqueue_shared(sessd_voxelattn* h, const sessd_tensor_desc* 
                                    const void* const* inputs, void* const* outputs, const void* window_workspace,
                                    sessd_stream_t stream);
 int sessd_voxelattn_set_flags(sessd_voxelattn* h, int32_t flags);
+/* workspace: where the windows lie that the call went by, another layer's for a sharer */
 int sessd_voxelattn_status(const sessd_voxelattn* h, const void* workspace, sessd_stream_t stream, int32_t* status);
 void sessd_voxelattn_destroy(sessd_voxelattn* h);
 

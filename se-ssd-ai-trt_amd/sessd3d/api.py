@@ -538,6 +538,7 @@ class Linear8(_Plugin):
 class VoxelAttention(_Plugin):
     """Attention among the voxels of a window of the grid: optional tanh cap of the scores, optional bias by distance."""
     kind = "voxelattn"
+    _list = None  # the workspace with the windows that the last call went by
 
     def __init__(self, num_heads, num_kv_heads, head_dim, spatial_shape_xyz, window_xyz, shift_xyz=(0, 0, 0), slopes=None,
                  cell_size_xyz=(1.0, 1.0, 1.0), cap=0.0, softmax_scale=0.0, max_voxels=B.MAX_VOXELS):
@@ -555,6 +556,23 @@ class VoxelAttention(_Plugin):
         self.max_voxels, self.cout = max_voxels, num_heads * head_dim
         self.windows = _windows_key(max_voxels, spatial_shape_xyz, window_xyz, shift_xyz)
 
+    def _enqueue_bound(self, bound, inputs, outputs, stream, workspace=None):
+        self._list = super()._enqueue_bound(bound, inputs, outputs, stream, workspace)
+        return self._list
+
+    def status(self, stream=None) -> int:
+        """Of the last call: of the list of windows that it went by, its own or another layer's."""
+        if self._list is None:
+            raise SessdError("voxelattn.status: the layer has not run")
+        s = C.c_int32(0)
+        check(self._fn("status")(self.h, _ptr(self._list), _stream_ptr(stream), C.byref(s)))
+        return s.value
+
+    def clone(self):
+        obj = super().clone()
+        obj._list = None
+        return obj
+
     def __call__(self, qkv, coors, voxel_num, stream=None, windows_from=None):
         """qkv [max_voxels, (num_heads + 2 num_kv_heads) * head_dim] -> [max_voxels, num_heads * head_dim].  windows_from: a layer on
         the same coordinates and windows that has run on this stream."""
@@ -571,6 +589,7 @@ class VoxelAttention(_Plugin):
                                  % (windows_from.windows, self.windows))
             check(lib().sessd_voxelattn_enqueue_shared(self.h, bound.ins, bound.outs, _pointers(ins), _pointers(outs),
                                                        _ptr(windows_from.ws), _stream_ptr(stream)))
+            self._list = windows_from.ws
         return out
 
 

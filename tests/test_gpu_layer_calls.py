@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from gpu_util import DEV, dev
-from sessd3d import api
+from sessd3d import api, ctypes_defs as D
 
 pytestmark = pytest.mark.gpu
 HALF, FLOAT = torch.float16, torch.float32
@@ -65,3 +65,39 @@ def test_a_captured_call_has_a_new_epilogue_as_a_whole():
         op.enqueue([q, s, n], [out])
         torch.cuda.synchronize()
         assert torch.equal(out, replayed) and bool((out < 0).any()) != relu
+
+
+def attention(rows, window=(4, 6, 6), heads=2, dim=16, **kw):
+    return api.VoxelAttention(heads, heads, dim, (50, 40, 9), window[::-1], max_voxels=rows, **kw)
+
+
+def attention_inputs(rows, heads=2, dim=16, seed=0, dtype=np.float16):
+    rng = np.random.default_rng(seed)
+    coors = np.zeros((rows, 4), np.int32)
+    at = rng.choice(9 * 40 * 50, rows, replace=False)
+    coors[:, 1], coors[:, 2], coors[:, 3] = at // 2000, at // 50 % 40, at % 50
+    return dev(rng.standard_normal((rows, 3 * heads * dim)).astype(dtype)), dev(coors), num(rows)
+
+
+@pytest.mark.parametrize("rows", [700, 5000])
+def test_the_status_of_a_layer_on_shared_windows_is_that_of_those_windows(rows):
+    x, c, n = attention_inputs(rows)
+    first, second = attention(rows), attention(rows)
+    with pytest.raises(api.SessdError, match="has not run"):
+        second.status()
+    first(x, c, n)
+    second(x, c, n, windows_from=first)
+    assert second.status() == 0
+    bad = c.clone()
+    bad[5, 1] = 9
+    first(x, bad, n)
+    second(x, bad, n, windows_from=first)
+    assert second.status() == D.SESSD_STATUS_BAD_COORD
+    second(x, c, n)          # alone again
+    assert second.status() == 0 and first.status() == D.SESSD_STATUS_BAD_COORD
+    ws = torch.empty_like(first.ws)
+    out = torch.empty((rows, 32), dtype=HALF, device=DEV)
+    second.enqueue([x, bad, n], [out], workspace=ws)
+    assert second.status() == D.SESSD_STATUS_BAD_COORD
+    with pytest.raises(api.SessdError, match="has not run"):
+        second.clone().status()
