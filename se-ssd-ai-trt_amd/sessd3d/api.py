@@ -584,12 +584,14 @@ class VoxelAttention(_Plugin):
         if windows_from is None:
             self._enqueue_bound(bound, ins, outs, stream)
         else:
-            if windows_from.windows != self.windows or windows_from.ws is None:
-                raise SessdError("windows_from: a layer that has run on the same windows (max_voxels, grid, window, shift): %s, %s"
+            # (its workspace alone says nothing: a call that was refused has left it as it was allocated)
+            found = windows_from._list
+            if windows_from.windows != self.windows or found is None or found.device != qkv.device:
+                raise SessdError("windows_from: a layer that has run on this device and on the same windows (max_voxels, grid, window, shift): %s, %s"
                                  % (windows_from.windows, self.windows))
-            check(lib().sessd_voxelattn_enqueue_shared(self.h, bound.ins, bound.outs, _pointers(ins), _pointers(outs),
-                                                       _ptr(windows_from.ws), _stream_ptr(stream)))
-            self._list = windows_from.ws
+            check(lib().sessd_voxelattn_enqueue_shared(self.h, bound.ins, bound.outs, _pointers(ins), _pointers(outs), _ptr(found),
+                                                       _stream_ptr(stream)))
+            self._list = found
         return out
 
 

@@ -101,3 +101,30 @@ def test_the_status_of_a_layer_on_shared_windows_is_that_of_those_windows(rows):
     assert second.status() == D.SESSD_STATUS_BAD_COORD
     with pytest.raises(api.SessdError, match="has not run"):
         second.clone().status()
+
+
+@pytest.mark.parametrize("rows", [700, 5000])
+def test_windows_of_a_call_that_was_refused_are_not_shared(rows):
+    x, c, n = attention_inputs(rows)
+    first, second, third = attention(rows), attention(rows), attention(rows)
+    odd = torch.empty(x.numel() + 1, dtype=HALF, device=DEV)[1:].reshape(x.shape)
+    with pytest.raises(api.SessdError, match="aligned"):
+        first(odd, c, n)
+    for layer in (first, first.clone()):
+        with pytest.raises(api.SessdError, match="windows_from"):
+            second(x, c, n, windows_from=layer)
+    want = first(x, c, n)
+    with pytest.raises(api.SessdError, match="windows_from"):
+        second(x, c, n, windows_from=first.clone())
+    with pytest.raises(api.SessdError, match="aligned"):
+        second(odd, c, n, windows_from=first)
+    with pytest.raises(api.SessdError, match="windows_from"):
+        third(x, c, n, windows_from=second)
+    # a sharer's windows can be shared, and so can those in a workspace of the caller's
+    assert torch.equal(second(x, c, n, windows_from=first), want) and torch.equal(third(x, c, n, windows_from=second), want)
+    ws, out = torch.empty_like(first.ws), torch.empty_like(want)
+    y, d, m = attention_inputs(rows, seed=1)
+    third.configure([y, d, m], [out])
+    third.enqueue([y, d, m], [out], workspace=ws)
+    first.ws.fill_(0x55)   # (what third's earlier calls went by)
+    assert torch.equal(second(y, d, m, windows_from=third), out)
