@@ -332,7 +332,8 @@ void sessd_sparse2dense_destroy(sessd_sparse2dense* h);
  * bits, the projection that reads such rows, and attention among the voxels of a window.  Life cycle, tensors, streams
  * and errors are those of the layers above; the first two need no workspace (workspace_size is 0, NULL is accepted).
  * Rows beyond voxel_num: zeros, or what Linear8's epilogue makes of zeros; left as they were with
- * SESSD_FLAG_SKIP_PAD_ROWS.  max_voxels: up to 2^24.  Outputs must not overlap inputs, but for RmsNorm's sum. */
+ * SESSD_FLAG_SKIP_PAD_ROWS.  max_voxels: up to 2^24.  Outputs must not overlap inputs, but for RmsNorm's sum.  A layer is
+ * bound to the device that is current when it is made: enqueue and set_epilogue with another current device are refused. */
 
 /* inputs : 0 feat [1,max_voxels,C] f32|f16   1 voxel_num i32[1]   [2 residual, as feat]
  * outputs: 0 q fp8 [1,max_voxels,C]   1 scale f32 [1,max_voxels,1]   [2 sum, as feat]

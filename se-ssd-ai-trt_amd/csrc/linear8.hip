@@ -252,6 +252,7 @@ int Linear8Plugin::create(const sessd_linear8_desc& d, const float* weights, Lin
     p->in_channel_ = cin;
     p->out_channel_ = cout;
     p->max_voxels_ = d.max_voxels;
+    SESSD_HIP_TRY(hipGetDevice(&p->device_));
     p->weights_.assign(weights, weights + (size_t)cin * cout);
     p->wscale_.assign((size_t)cout, 0.f);
     for (int k = 0; k < cin; ++k)
@@ -304,6 +305,7 @@ int Linear8Plugin::uploadColumns(const Epilogue& e) {
 }
 
 int Linear8Plugin::setEpilogue(const float* scale, const float* shift, int relu) {
+    SESSD_TRY(check_device(device_, "linear8.set_epilogue"));
     Epilogue e;
     e.relu = relu ? 1 : 0;
     if (scale) e.scale_host.assign(scale, scale + out_channel_);
@@ -380,6 +382,7 @@ int Linear8Plugin::enqueue(const sessd_tensor_desc* inputDesc, const sessd_tenso
     SESSD_TRY(check(inputDesc, outputDesc));
     if ((reinterpret_cast<uintptr_t>(inputs[0]) | reinterpret_cast<uintptr_t>(inputs[1]) | reinterpret_cast<uintptr_t>(outputs[0])) & 15)
         return fail(SESSD_E_INVALID, "linear8.enqueue: tensors must be 16-byte aligned");
+    SESSD_TRY(check_device(device_, "linear8.enqueue"));
     LinearArgs a;
     a.q = static_cast<const uint8_t*>(inputs[0]);
     a.scale = static_cast<const float*>(inputs[1]);

@@ -298,6 +298,7 @@ class RmsNormPlugin {
     int type_ = SESSD_FLOAT;
     bool residual_ = false;  // configured with a third input
     int flags_ = 0;
+    int device_ = 0;
 
   private:
     int check(const sessd_tensor_desc* in, const sessd_tensor_desc* out, bool residual) const;
@@ -324,6 +325,7 @@ class Linear8Plugin {
     Epilogue epi_;                       // (host side; the device has it in columns_dev_)
     int out_type_ = SESSD_FLOAT;
     int flags_ = 0;
+    int device_ = 0;
 
   private:
     int check(const sessd_tensor_desc* in, const sessd_tensor_desc* out) const;
@@ -351,6 +353,7 @@ class VoxelAttentionPlugin {
     float* slopes_dev_ = nullptr;
     int type_ = SESSD_FLOAT;
     int flags_ = 0;
+    int device_ = 0;
 
   private:
     int check(const sessd_tensor_desc* in, const sessd_tensor_desc* out) const;
@@ -364,6 +367,8 @@ class VoxelAttentionPlugin {
 constexpr int kMostRows = 1 << 24;
 int check_rows(const sessd_tensor_desc& d, int max_voxels, int channels, const char* who, const char* what);
 bool is_scalar_int(const sessd_tensor_desc& d);
+// The device that a layer's weights are on is the one that was current when it was made; its kernels run on no other.
+int check_device(int device, const char* who);
 
 // little-endian field (de)serialisation in declaration order, as the reference's
 // writeToBuffer / readFromBuffer (voxelGenerator.cu:44-58)

@@ -225,6 +225,13 @@ bool is_scalar_int(const sessd_tensor_desc& d) {
     return d.type == SESSD_INT32;
 }
 
+int check_device(int device, const char* who) {
+    int current = 0;
+    SESSD_HIP_TRY(hipGetDevice(&current));
+    if (current != device) return fail(SESSD_E_INVALID, "%s: the layer was made on device %d, the current one is %d", who, device, current);
+    return SESSD_OK;
+}
+
 RmsNormPlugin::~RmsNormPlugin() {
     if (gamma_dev_) (void)hipFree(gamma_dev_);
 }
@@ -241,6 +248,7 @@ int RmsNormPlugin::create(const sessd_rmsnorm_desc& d, const float* gamma, RmsNo
     p->max_voxels_ = d.max_voxels;
     p->eps_ = d.eps;
     p->gamma_.assign(gamma, gamma + d.channel);
+    SESSD_HIP_TRY(hipGetDevice(&p->device_));
     SESSD_HIP_TRY(hipMalloc(reinterpret_cast<void**>(&p->gamma_dev_), d.channel * sizeof(float)));
     SESSD_HIP_TRY(hipMemcpy(p->gamma_dev_, gamma, d.channel * sizeof(float), hipMemcpyHostToDevice));
     *out = p.release();
@@ -309,6 +317,7 @@ int RmsNormPlugin::enqueue(const sessd_tensor_desc* inputDesc, const sessd_tenso
     }
     if (inputDesc[0].type != type_) return fail(SESSD_E_INVALID, "rmsnorm.enqueue: tensor dtypes differ from the configured ones");
     SESSD_TRY(check(inputDesc, outputDesc, residual_));
+    SESSD_TRY(check_device(device_, "rmsnorm.enqueue"));
     NormArgs a;
     a.feat = inputs[0];
     a.residual = residual_ ? inputs[2] : nullptr;

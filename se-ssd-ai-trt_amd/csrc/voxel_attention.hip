@@ -64,6 +64,7 @@ int VoxelAttentionPlugin::create(const sessd_voxelattn_desc& d, const float* slo
         return fail(SESSD_E_UNSUPPORTED, "voxelattn: softmax_scale and score_cap must be 0 or 2^-40 .. 2^40, cell_size at most 2^20");
     std::unique_ptr<VoxelAttentionPlugin> p(new VoxelAttentionPlugin());
     p->desc_ = d;
+    SESSD_HIP_TRY(hipGetDevice(&p->device_));
     if (slopes) {
         for (int h = 0; h < d.num_heads; ++h) {
             if (!std::isfinite(slopes[h])) return fail(SESSD_E_INVALID, "voxelattn: the slopes must be finite");
@@ -132,7 +133,7 @@ int VoxelAttentionPlugin::checkCall(const sessd_tensor_desc* inputDesc, const se
     if ((reinterpret_cast<uintptr_t>(inputs[0]) | reinterpret_cast<uintptr_t>(inputs[1]) | reinterpret_cast<uintptr_t>(outputs[0]) |
          reinterpret_cast<uintptr_t>(workspace)) & 15)
         return fail(SESSD_E_INVALID, "%s: tensors and workspace must be 16-byte aligned", who);
-    return SESSD_OK;
+    return check_device(device_, who);
 }
 
 int VoxelAttentionPlugin::attend(const void* const* inputs, void* const* outputs, const void* workspace, hipStream_t stream) const {

@@ -92,6 +92,39 @@ def check_epilogue():
     L.sessd_linear8_destroy(lin.h)
 
 
+def check_device():
+    """A layer that was made on one device refuses calls while another is current."""
+    rows = 100
+    feat = [((1, rows, 48), F16), ((1,), I32)]
+    h = C.c_void_p()
+    g = np.ones(48, np.float32)
+    assert L.sessd_rmsnorm_create(C.byref(D.RmsNormDesc(48, rows, 1e-6)), g.ctypes.data, C.byref(h)) == 0
+    i, o = descs(*feat), descs(((1, rows, 48), FP8), ((1, rows, 1), F32))
+    assert L.sessd_rmsnorm_configure(h, i, 2, o, 2) == 0
+    a = C.c_void_p()
+    d = D.VoxelAttnDesc(2, 2, 8, rows, (C.c_int32 * 3)(20, 20, 4), (C.c_int32 * 3)(5, 5, 4), (C.c_int32 * 3)(), (C.c_float * 3)(1, 1, 1), 0, 0)
+    assert L.sessd_voxelattn_create(C.byref(d), None, C.byref(a)) == 0
+    ai, ao = descs(((1, rows, 48), F16), ((1, rows, 4), I32), ((1,), I32)), descs(((1, rows, 16), F16))
+    assert L.sessd_voxelattn_configure(a, ai, 3, ao, 1) == 0
+    FAKE.fake_set_device(2)
+    lin = Linear(32, 20, np.ones((32, 20)))
+    calls = [lambda: L.sessd_rmsnorm_enqueue(h, i, o, pointers(4096, 64), pointers(8192, 16384), None, None),
+             lambda: L.sessd_voxelattn_enqueue(a, ai, ao, pointers(4096, 8192, 64), pointers(16384), 65536, None),
+             lambda: L.sessd_voxelattn_enqueue_shared(a, ai, ao, pointers(4096, 8192, 64), pointers(16384), 65536, None)]
+    own = [lin.call, lambda: lin.set_epilogue(None, np.ones(20), 1)]
+    for device in (2, 0, 1, 0, 2):
+        FAKE.fake_set_device(device)
+        for call, made in [(c, 0) for c in calls] + [(c, 2) for c in own]:
+            log()
+            rc, text = call(), L.sessd_last_error().decode()
+            if made == device:
+                assert rc == 0
+            else:
+                assert rc == D.SESSD_E_INVALID and "device %d" % made in text and "one is %d" % device in text, text
+                assert not log()
+    FAKE.fake_set_device(0)
+
+
 CHECKS = {k[6:]: v for k, v in list(globals().items()) if k.startswith("check_")}
 
 if __name__ == "__main__":
