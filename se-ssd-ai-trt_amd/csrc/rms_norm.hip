@@ -133,7 +133,17 @@ rms_norm(const T* feat, const T* residual, const float* __restrict__ gamma, cons
 #pragma unroll
     for (int d = LANES / 2; d > 0; d /= 2) squares += __shfl_xor(squares, d);
     const float mean = squares / (float)channel + eps;
-    const float rms = 1.f / sqrtf(mean);
+    double rms = 1.f / sqrtf(mean);
+    if (mean < 0x1p-100f) {  // (eps is as small: the squares are at the end of FP32, or beyond it)
+        double sum64 = 0.;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) sum64 = fma((double)h[j][e], (double)h[j][e], sum64);
+#pragma unroll
+        for (int d = LANES / 2; d > 0; d /= 2) sum64 += __shfl_xor(sum64, d);
+        rms = 1. / sqrt(sum64 / channel + (double)eps);
+    }
     float g[NV][VEC];
     double most = 0.;  // of |gamma h|, exact
 #pragma unroll
@@ -148,14 +158,14 @@ rms_norm(const T* feat, const T* residual, const float* __restrict__ gamma, cons
     }
 #pragma unroll
     for (int d = LANES / 2; d > 0; d /= 2) most = fmax(most, __shfl_xor(most, d));
-    float s = (float)(most * (double)rms / (double)kMost);
+    float s = (float)(most * rms / (double)kMost);
     double by = (double)kMost / most;
     if (!(s > kSmallestScale)) {
         s = kSmallestScale;
-        by = (double)rms / (double)kSmallestScale;
+        by = rms / (double)kSmallestScale;
     }
     // fmax() drops NaN: whether the row had something that is not finite shows in its sum of squares
-    if (!(mean <= FLT_MAX && rms <= FLT_MAX && s <= FLT_MAX)) {
+    if (!(mean <= FLT_MAX && rms <= DBL_MAX && s <= FLT_MAX)) {
         s = __int_as_float(0x7fc00000);
         by = (double)s;
     }
