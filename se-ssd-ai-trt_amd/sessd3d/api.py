@@ -493,6 +493,13 @@ class RmsNorm(_Plugin):
         super().__init__(h)
         self.max_voxels, self.channel = max_voxels, channel
 
+    @classmethod
+    def deserialize(cls, blob: bytes):
+        obj = super().deserialize(blob)
+        d = D.RmsNormDesc.from_buffer_copy(blob)
+        obj.max_voxels, obj.channel = d.max_voxels, d.channel
+        return obj
+
     def __call__(self, feat, voxel_num, residual=None, stream=None):
         """feat, residual [max_voxels, channel] -> q float8_e4m3fn, scale f32 [max_voxels, 1] (, sum as feat, with a residual)"""
         torch = _torch()
@@ -518,6 +525,13 @@ class Linear8(_Plugin):
         check(lib().sessd_linear8_create(C.byref(d), _np_f32_ptr(w), C.byref(h)))
         super().__init__(h)
         self.max_voxels, self.cout = max_voxels, out_channel
+
+    @classmethod
+    def deserialize(cls, blob: bytes):
+        obj = super().deserialize(blob)
+        d = D.Linear8Desc.from_buffer_copy(blob)
+        obj.max_voxels, obj.cout = d.max_voxels, d.out_channel
+        return obj
 
     def set_epilogue(self, scale=None, shift=None, relu=True):
         sc = None if scale is None else np.ascontiguousarray(scale, np.float32)
@@ -555,6 +569,14 @@ class VoxelAttention(_Plugin):
         super().__init__(h)
         self.max_voxels, self.cout = max_voxels, num_heads * head_dim
         self.windows = _windows_key(max_voxels, spatial_shape_xyz, window_xyz, shift_xyz)
+
+    @classmethod
+    def deserialize(cls, blob: bytes):
+        obj = super().deserialize(blob)
+        d = D.VoxelAttnDesc.from_buffer_copy(blob)
+        obj.max_voxels, obj.cout = d.max_voxels, d.num_heads * d.head_dim
+        obj.windows = _windows_key(d.max_voxels, d.spatial_shape, d.window_shape, d.window_shift)
+        return obj
 
     def _enqueue_bound(self, bound, inputs, outputs, stream, workspace=None):
         self._list = super()._enqueue_bound(bound, inputs, outputs, stream, workspace)

@@ -128,3 +128,19 @@ def test_windows_of_a_call_that_was_refused_are_not_shared(rows):
     third.enqueue([y, d, m], [out], workspace=ws)
     first.ws.fill_(0x55)   # (what third's earlier calls went by)
     assert torch.equal(second(y, d, m, windows_from=third), out)
+
+
+def test_layers_read_back_from_their_bytes_are_called_as_the_first_ones():
+    rng = np.random.default_rng(0)
+    rows = 300
+    x, c, n = attention_inputs(rows)
+    attn = attention(rows, slopes=[1.0, 0.5], cap=20.0, cell_size_xyz=(0.1, 0.1, 0.2))
+    again = api.VoxelAttention.deserialize(attn.serialize())
+    want = attn(x, c, n)
+    assert torch.equal(again(x, c, n), want) and torch.equal(again(x, c, n, windows_from=attn), want)
+    norm = api.RmsNorm(96, rng.uniform(0.5, 1.5, 96).astype(np.float32), max_voxels=rows)
+    a, b = norm(x, n), api.RmsNorm.deserialize(norm.serialize())(x, n)
+    assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(a, b))
+    lin = api.Linear8(96, 40, rng.standard_normal((96, 40)).astype(np.float32), max_voxels=rows)
+    lin.set_epilogue(None, rng.standard_normal(40).astype(np.float32), relu=True)
+    assert torch.equal(api.Linear8.deserialize(lin.serialize())(*a, n), lin(*a, n))
