@@ -53,3 +53,20 @@ def one_window(qkv, cells, heads, kv_heads, dim, slopes=None, cell=(1.0, 1.0, 1.
             tol = tol + np.abs(o) * 4 * U
         out[:, h * dim:(h + 1) * dim], bound[:, h * dim:(h + 1) * dim] = o, tol
     return out, bound
+
+
+def windows(qkv, cells, window, heads, kv_heads, dim, most=1000, seed=0, **kw):
+    """The same for rows of several windows: rows that are checked, output, bound.  Of a window of more than `most` rows, 150 are."""
+    _, which = np.unique(cells // np.array(window), axis=0, return_inverse=True)
+    which = which.reshape(-1)
+    rows, outs, bounds = [], [], []
+    for w in range(which.max() + 1):
+        at = np.nonzero(which == w)[0]
+        some = None
+        if len(at) > most:
+            some = np.unique(np.concatenate([[0, len(at) - 1], np.random.default_rng(seed).integers(len(at), size=150)]))
+        o, b = one_window(qkv[at], cells[at], heads, kv_heads, dim, queries=some, **kw)
+        rows.append(at if some is None else at[some])
+        outs.append(o)
+        bounds.append(b)
+    return np.concatenate(rows), np.concatenate(outs), np.concatenate(bounds)
