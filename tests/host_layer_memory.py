@@ -125,6 +125,54 @@ def check_device():
     FAKE.fake_set_device(0)
 
 
+def check_weights():
+    """The weights that the GPU has are the e4m3 nearest to W / wscale, widened to halves, each where the instructions want it: of 16 columns times 32
+    channels, lane l has column l % 16 and the eight channels of its quarter; columns are dealt so that a lane's results are neighbours."""
+    import layer_oracle as O
+    rng = np.random.default_rng(0)
+    for cin, cout in ((16, 5), (48, 70), (256, 64), (272, 33), (512, 40), (1040, 100)):
+        w = (rng.standard_normal((cin, cout)) * 10.0 ** rng.uniform(-20, 20, cout)).astype(np.float32)
+        w[:, 3] = 0
+        w[0, 1:3] = 448 * np.abs(w[:, 1:3]).max()     # (a scale of which ties and the values below 2^-6 are reached)
+        w[1:16, 1] = w[0, 1] / 448 * np.arange(1, 16) * 2.0 ** -10
+        w[1:16, 2] = w[0, 2] / 448 * (16.5 + np.arange(15))
+        wscale = np.maximum(np.abs(w).max(0) / np.float32(448), np.float32(2.0 ** -100)).astype(np.float32)
+        codes = O.to_e4m3(w / wscale)
+        lin = Linear(cin, cout, w)
+        (p, size), (cp, csize) = lin.memory
+        tiles = 2 if 256 < cin <= 512 else 4
+        blocks, steps = -(-cout // (16 * tiles)), 2 * -(-cin // 64)
+        halves = np.frombuffer(C.string_at(p, size), np.float16).reshape(2, blocks, steps, tiles, 64, 8)  # FP32 outputs, FP16 ones
+        seen = np.zeros((2, cin, cout), int)
+        for half in (0, 1):
+            for b in range(blocks):
+                for s in range(steps):
+                    for t in range(tiles):
+                        for lane in range(64):
+                            r, g = lane % 16, lane // 16
+                            # of instruction t, results 4 (r / 4) .. + 3 go to one lane: FP16 stores 8 of a pair of instructions, FP32 4 of one
+                            col = b * 16 * tiles + ((t // 2) * 32 + (r // 4) * 8 + (t % 2) * 4 + r % 4 if half else t * 16 + r)
+                            for e in range(8):
+                                ch = (s // 2) * 64 + g * 16 + (s % 2) * 8 + e   # (a lane reads 16 neighbouring bytes of a row for two steps)
+                                got = float(halves[half, b, s, t, lane, e])
+                                if col < cout and ch < cin:
+                                    assert got == O.VALUES[codes[ch, col]], (cin, cout, half, ch, col, got)
+                                    seen[half, ch, col] += 1
+                                else:
+                                    assert got == 0
+        assert (seen == 1).all()
+        pad = blocks * 16 * tiles
+        sc, sh = rng.standard_normal((2, cout)).astype(np.float32)
+        for scale, shift, relu in ((None, None, None), (sc, sh, 1), (None, sh, 0), (sc, None, 1)):
+            if relu is not None:
+                assert lin.set_epilogue(scale, shift, relu) == 0
+            columns = np.frombuffer(C.string_at(cp, csize), np.float32)
+            assert np.array_equal(columns[:cout], wscale if scale is None else wscale * scale) and not columns[cout:pad].any()
+            assert np.array_equal(columns[pad:pad + cout], np.zeros(cout) if shift is None else shift) and not columns[pad + cout:2 * pad].any()
+            assert columns[2 * pad] == (relu or 0)
+        L.sessd_linear8_destroy(lin.h)
+
+
 CHECKS = {k[6:]: v for k, v in list(globals().items()) if k.startswith("check_")}
 
 if __name__ == "__main__":
