@@ -629,9 +629,28 @@ def plugin_field_names(plugin_name):
             for i in range(fc.contents.nbFields)]
 
 
+# Of this library's own layers: the weights' field, and the fields whose product is how many values it has
+_OWN_WEIGHTS = {"RmsNormPlugin": ("gamma", ("channel",)), "Linear8Plugin": ("weights", ("in_channel", "out_channel")),
+                "VoxelAttentionPlugin": ("slopes", ("num_heads",))}
+
+
+def _check_field_sizes(plugin_name, fields):
+    """The creators take a field of length 1 for one of which the length is not known, and read what they need.  Here it is known."""
+    weights, of = _OWN_WEIGHTS[plugin_name]
+    for name, _, length in plugin_field_names(plugin_name):
+        if name not in fields or (name == weights and not all(k in fields for k in of)):
+            continue  # (the creator names the field that is missing)
+        if name == weights:
+            length = int(np.prod([int(np.asarray(fields[k]).reshape(-1)[0]) for k in of]))
+        if np.asarray(fields[name]).size != length:
+            raise SessdError("%s: field '%s' holds %d values, the layer needs %d" % (plugin_name, name, np.asarray(fields[name]).size, length))
+
+
 def create_plugin(plugin_name, fields):
     """createPlugin(name, PluginFieldCollection) of the reference's creators: `fields` maps field names to numpy
     arrays (int32 or float32).  -> the wrapper object of that plugin type."""
+    if plugin_name in _OWN_WEIGHTS:
+        _check_field_sizes(plugin_name, fields)
     keep = []
     arr = (D.PluginField * max(len(fields), 1))()
     for i, (k, v) in enumerate(fields.items()):

@@ -173,6 +173,28 @@ def check_weights():
         L.sessd_linear8_destroy(lin.h)
 
 
+def check_fields():
+    """Fields that hold fewer values than the layer has are refused, those with a single one as well."""
+    i = lambda *v: np.array(v, np.int32)  # noqa: E731
+    f = lambda *v: np.array(v, np.float32)  # noqa: E731
+    three = dict(spatial_shape=i(20, 20, 4), window_shape=i(5, 5, 4), window_shift=i(0, 0, 0), cell_size=f(1, 1, 1))
+    plugins = {"RmsNormPlugin": dict(channel=i(48), max_voxels=i(100), eps=f(1e-6), gamma=f(*[1] * 48)),
+               "Linear8Plugin": dict(in_channel=i(32), out_channel=i(20), max_voxels=i(100), weights=f(*[1] * 640)),
+               "VoxelAttentionPlugin": dict(num_heads=i(4), num_kv_heads=i(2), head_dim=i(16), max_voxels=i(100), softmax_scale=f(0), score_cap=f(0),
+                                            slopes=f(1, 2, 3, 4), **three)}
+    for name, fields in plugins.items():
+        assert api.create_plugin(name, fields).max_voxels == 100
+        for key, v in fields.items():
+            for bad in (v[:1], v[:-1], v[:0], np.concatenate([v, v])):
+                if bad.size == v.size:
+                    continue
+                try:
+                    api.create_plugin(name, dict(fields, **{key: bad}))
+                    raise AssertionError((name, key))
+                except api.SessdError as e:
+                    assert key in str(e), e
+
+
 CHECKS = {k[6:]: v for k, v in list(globals().items()) if k.startswith("check_")}
 
 if __name__ == "__main__":

@@ -21,7 +21,7 @@ def fake_hip(tmp_path_factory):
     return out
 
 
-@pytest.mark.parametrize("check", ["epilogue", "device", "weights"])
+@pytest.mark.parametrize("check", ["epilogue", "device", "weights", "fields"])
 def test_device_memory(fake_hip, check):
     r = subprocess.run([sys.executable, os.path.join(HERE, "host_layer_memory.py"), fake_hip, check], stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
                        text=True, timeout=300)
