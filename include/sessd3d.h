@@ -338,9 +338,10 @@ void sessd_sparse2dense_destroy(sessd_sparse2dense* h);
 /* inputs : 0 feat [1,max_voxels,C] f32|f16   1 voxel_num i32[1]   [2 residual, as feat]
  * outputs: 0 q fp8 [1,max_voxels,C]   1 scale f32 [1,max_voxels,1]   [2 sum, as feat]
  * h = feat + residual, y = gamma * h / sqrt(mean over C of h^2 + eps), scale = max(max|y| / 448, 2^-100),
- * q = y / scale to the nearest e4m3, sum = h.  All of it is computed in FP32 from the unrounded h.  A row with a value
- * that is not finite, or whose mean of h^2 is not (|h| from about 1e19), leaves nothing that counts: its scale is NaN and
- * all of its q are.  `sum` may be the tensor `feat` or `residual`.
+ * q = y / scale to the nearest e4m3, sum = h.  From the unrounded h: sums, mean, root and scale in FP32 (in 64 bits where FP32
+ * does not hold the squares because they are small), the quotient q in 64 bits.  A row with a value that is not finite, or
+ * whose mean of h^2 (|h| from about 1e19) or scale is not, leaves nothing that counts: its scale is NaN and all of its q
+ * are; so does a row of zeros with eps = 0.  `sum` may be the tensor `feat` or `residual`.
  * With two inputs there are two outputs, with three three.  channel: 1 .. 4096, multiples of 8 are fastest. */
 typedef struct sessd_rmsnorm sessd_rmsnorm;
 
@@ -400,7 +401,8 @@ void sessd_linear8_destroy(sessd_linear8* h);
  *     score = softmax_scale * q_i . k_j;   score = score_cap * tanh(score / score_cap) if score_cap > 0;
  *     score -= slope[h] * |p_i - p_j|,  p = coor * cell_size (Euclidean distance of the voxels' centres);
  *     feat_i = sum over j of softmax_j(score) * v_j
- * Scores, softmax and sums are FP32; with FP16 tensors the weights are rounded to FP16 in front of their product with v.
+ * Scores, softmax and sums are FP32, distances those of whole cells; with FP16 tensors the weights, times 2^14, are rounded
+ * to FP16 in front of their product with v: 11 bits, down to 2^-39 of a row's largest.
  * A row whose coordinates lie outside the grid takes part in nothing, its output is zeros and SESSD_STATUS_BAD_COORD is
  * raised.  Rows that name one voxel are all of them rows of its window.  No value of another window reaches a row, whatever
  * it is.  The order of a row's sums follows from its window's rows, ascending, and the layer's own sizes: a row's bits do not
@@ -433,7 +435,8 @@ int sessd_voxelattn_enqueue(sessd_voxelattn* h, const sessd_tensor_desc* inDesc,
 /* The layer on the windows that an earlier sessd_voxelattn_enqueue left in `window_workspace` (same coors, voxel_num,
  * max_voxels, spatial_shape, window_shape and window_shift; heads, slopes and the rest may differ): consecutive layers on
  * one coors tensor find their windows once.  The same bits as sessd_voxelattn_enqueue.  The rows that there are, are those of
- * the earlier call, whatever coors and voxel_num hold by now. */
+ * the earlier call, whatever coors and voxel_num hold by now.  That call must have run, or be in front on the stream: one
+ * that a graph has captured has not until the graph is replayed. */
 int sessd_voxelattn_enqueue_shared(sessd_voxelattn* h, const sessd_tensor_desc* inDesc, const sessd_tensor_desc* outDesc,
                                    const void* const* inputs, void* const* outputs, const void* window_workspace,
                                    sessd_stream_t stream);

@@ -11,9 +11,9 @@
 // Up to kMostHeld input channels a wave keeps the weights of its columns (64, or 32 where the channels are many) in registers, 128 of
 // them at most, and takes one block of 16 rows after the other, the next one's values requested while it multiplies: nothing of the
 // weights is read twice, nothing goes through LDS but the epilogue's constants, and no wave waits for another.  The waves of a
-// workgroup have neighbouring columns of the same rows.  What bounds it then is the output it writes: 150 000 rows 256 -> 1024 FP16 104 us, 3.5 TB/s and
-// 760 TFLOP/s; 60 000 rows 512 -> 128 FP32 21 us; weights read anew for every 16 rows 359 and 44 us.  Inputs beyond kMostHeld, whose weights no
-// wave's registers hold, do read them anew.
+// workgroup have neighbouring columns of the same rows.  What bounds it then is the output it writes: 150 000 rows 256 -> 1024 FP16 102 us, 3.6 TB/s and
+// 770 TFLOP/s; 60 000 rows 512 -> 128 FP32, 7.3 blocks for each wave, 21 us; weights read anew for every 16 rows 266 and 30 us.  Inputs beyond
+// kMostHeld, whose weights no wave's registers hold, do read them anew: 150 000 rows 1024 -> 256 FP16 248 us, 60 000 rows 2048 -> 512 FP32 368.
 #include <cmath>
 #include <utility>
 
@@ -58,7 +58,7 @@ struct LinearArgs {
     void* out;
 };
 
-// (past the caches: 150 000 x 256 -> 1024 150 us through them, 107 like this)
+// (past the caches: 150 000 x 256 -> 1024 150 us through them, 102 like this)
 template <typename V>
 __device__ __forceinline__ void put(V* to, const V& x) {
     __builtin_nontemporal_store(x, to);

@@ -6,9 +6,9 @@
 // 32 rows are a wave's own affair: their queries are their keys, which it keeps in registers, and nobody waits for anybody.  Where there are
 // few queries, a workgroup has 16 of them and its waves share the keys out (shared_rows).
 //
-// What bounds it are vector instructions, 55 to 88 cycles for a wave's 64 scores (a distance 40, a cap 28, exponential, maximum and sums 26), not the
-// matrix cores, nor memory: 30 000 keys, 8 heads of 64 values, cap and distances 5.2 ms (350 TFLOP/s of products), 53 000 rows in windows of 16 x 16, 8 heads
-// of 32 98 us; FP32, where the products take longer, 5 111 keys, 16 heads of 64 1.23 ms (82 TFLOP/s).
+// What bounds it are vector instructions, 56 to 110 cycles for a wave's 64 scores (a distance 52, which two heads may share, a cap 28, exponential,
+// maximum and sums 30), not the matrix cores, nor memory: 30 000 keys, 8 heads of 64 values, cap and distances 5.3 ms (350 TFLOP/s of products),
+// 53 000 rows in windows of 16 x 16, 8 heads of 32 102 us; FP32, where the products take longer, 4 741 keys, 16 heads of 64 1.27 ms (73 TFLOP/s).
 //
 // Scores are taken transposed, S^T = K Q^T: a lane of the result has one query (its column) and four keys, so that maximum and sum over the
 // keys are mostly the lane's own, and the weights are where the second product, O^T = V^T P^T, wants them.  Maximum and sum run along
@@ -208,18 +208,20 @@ struct AttentionShape {
     using Type = T;
     using Op = Operand<T, DP>;
     static constexpr int kDim = DP, HG = HG_, KVG = KVG_, KB = KB_;
-    // 16 keys each, that a wave takes at once (two heads of 64 values: 6.1 ms at 30 000 keys with 4, 5.8 with 2, whose sums leave registers, both with two waves a SIMD)
+    // 16 keys each, that a wave takes at once (two heads of 64 values: 6.4 ms at 30 000 keys with 4, 6.2 with 2, whose sums leave registers,
+    // both with two waves a SIMD)
     static constexpr int H = KB == 64 && HG * DP < 128 ? 4 : 2;
     static constexpr int kHalf = KVG * KB * Op::kPitch;                                  // keys, or values, in LDS
     static constexpr int kTiny = kAttentionBlock / 64 * kTinyRows * Op::kPitch;          // the values of a tiny window for each wave
     static constexpr int kWordsHead = DP / Op::kPer;                                     // 16-byte words of a head's row
     static constexpr int kLoads = (2 * KVG * kWordsHead * KB + kAttentionBlock - 1) / kAttentionBlock;  // of a thread
-    // Where the waves of a workgroup share the keys out: keys of a wave's block (up to eight words of a lane), its keys and values in LDS
+    // Where the waves of a workgroup share the keys out: keys of a wave's block (eight words of a lane, sixteen in FP32 with heads
+    // of 128 values), its keys and values in LDS
     static constexpr int KW = 256 / kWordsHead > 64 ? 64 : 256 / kWordsHead < 16 ? 16 : 256 / kWordsHead;
     static constexpr int kWave = 2 * KW * Op::kPitch;
     // Waves of a SIMD that the registers leave room for.  A third one is worth a few registers in memory: 30 000 keys, 8 heads of 64 values on 4 of keys
-    // 5.9 -> 5.4 ms, few rows 4 096 and 16 heads of 64 values in FP32 943 -> 830 us, 4 096 and 8 of 64 in FP16 194 -> 179.  Kernels that keep to 168
-    // by themselves are scheduled worse under the bound (53 000 rows, 8 heads of 32: 102 -> 106), those beyond 180 lose too many.
+    // 6.2 -> 5.3 ms, few rows 3 800 and 16 heads of 64 values in FP32 948 -> 831 us, 3 800 and 8 of 64 in FP16 202 -> 177.  Kernels that keep to 168
+    // by themselves are scheduled worse under the bound (53 000 rows, 8 heads of 32: 106 -> 110), those beyond 180 lose too many.
     static constexpr int kWavesListed = DP == 64 && HG == 2 && KVG == 1 ? 3 : 2, kWavesFew = DP <= 64 ? 3 : 2;
 };
 
@@ -664,8 +666,8 @@ voxel_attention(AttentionArgs a) {
 // among them and the blocks of 64 queries (16, SHARED) that do.
 constexpr int kFewPlaces = 16;
 // Waves that share a query's keys reach four times as much of the card with few queries, but read each key for 16 queries instead of 64 and have more
-// registers.  FP16, 64 and 16 queries a workgroup: 1 951 rows of one window and 2 heads of 16 values 45 and 21 us, 4 096 and 8 of 64 415 and 193, but 24 of
-// 64 430 and 520, and windows of 60 rows at 4 096 rows and 16 heads 28 and 40.  FP32, whose products take longer: 4 096 rows and 16 heads of 64 1 509 and 936.
+// registers.  FP16, 64 and 16 queries a workgroup: 1 866 rows of one window and 2 heads of 16 values 47 and 21 us, 3 800 and 8 of 64 431 and 177, but 24 of
+// 64 439 and 468, and windows of 6 x 6 at 3 800 rows and 16 heads 30 and 37.  FP32, whose products take longer: 3 800 rows and 16 heads of 64 1 480 and 831.
 constexpr int kSharedRows = 32768;  // rows times heads, FP16
 template <typename S, int CAP, bool BIAS, bool SHARED>
 __global__ void __launch_bounds__(kAttentionBlock, S::kWavesFew)
@@ -752,9 +754,10 @@ inline int kv_heads_of(const AttentionArgs& a, int group) {
 // What a thread keeps of the next block are eight words at most.
 template <typename T, int DP, int KB>
 void launch_attention_dim(const AttentionArgs& a, hipStream_t stream) {
-    // A second head uses the distances of the first; a wave's registers leave the card fewer waves.  FP16, HG 1 and 2: 16 000 voxels times 8
-    // heads of 16 values 38.7 and 40.7 us, 14 000 times 16 of 16 43.9 and 48.4, 12 000 times 16 of 32 78 and 68, 53 000 times 8 of 32 135 and 101,
-    // 30 000 times 8 of 64 in one window 6.9 and 5.3 ms (with cap).  FP32 waits for the matrix cores: 61 and 77 us.
+    // A second head uses the distances of the first; a wave's registers leave the card fewer waves.  FP16, HG 1 and 2: 7 200 voxels of one window times
+    // 16 heads of 32 values 622 and 760 us, 16 000 in windows times 8 of 16 42.5 and 49, 12 000 times 16 of 16 44.5 and 49.7, 10 300 times 16 of 32 82
+    // and 84, 53 000 times 8 of 32 142 and 106, 30 000 times 8 of 64 in one window 7.1 and 5.3 ms (with cap).  FP32 waits for the matrix cores:
+    // 16 000 times 8 of 24 62 and 80 us.
     if constexpr (sizeof(T) == 2) {
         if ((int64_t)a.w.max_voxels * a.heads >= 200000) {
             if (kv_heads_of(a, 2) == 1) return launch_attention_shape<AttentionShape<T, DP, 2, 1, KB>>(a, stream);

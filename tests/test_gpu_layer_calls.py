@@ -39,7 +39,10 @@ def test_a_new_epilogue_waits_for_the_calls_that_have_the_old_one(cin, cout):
     torch.cuda.synchronize()
     with torch.cuda.stream(side):
         queued = [op(q, s, n) for _ in range(12)]
+        done = torch.cuda.Event()
+        done.record()
         op.set_epilogue(new[0], new[1], relu=new[2])
+        assert done.query()
         behind = op(q, s, n)
     torch.cuda.synchronize()
     assert all(torch.equal(x, want[1]) for x in queued) and torch.equal(behind, want[0])
