@@ -475,6 +475,12 @@ def _dense(*tensors):
         raise SessdError("the tensors are on device %d, the current one is %d" % (device, _current_device()))
 
 
+def _another_stream(stream):
+    """Whether this is a stream of torch's that is not the current one.  What a call on it allocates is memory of that stream: memory that was last
+    used on the current one may still be read there."""
+    return stream is not None and isinstance(stream, _torch().cuda.Stream) and stream.cuda_stream != _stream_ptr()
+
+
 def _windows_key(max_voxels, spatial_shape, window, shift):
     """What two layers have alike that share their windows."""
     return (int(max_voxels),) + tuple(tuple(int(v) for v in a) for a in (spatial_shape, window, shift))
@@ -503,6 +509,9 @@ class RmsNorm(_Plugin):
     def __call__(self, feat, voxel_num, residual=None, stream=None):
         """feat, residual [max_voxels, channel] -> q float8_e4m3fn, scale f32 [max_voxels, 1] (, sum as feat, with a residual)"""
         torch = _torch()
+        if _another_stream(stream):
+            with torch.cuda.stream(stream):
+                return self(feat, voxel_num, residual)
         ins = (feat, voxel_num) if residual is None else (feat, voxel_num, residual)
         _dense(*ins)
         # (outputs like feat: where that has another shape than the layer, configure says so)
@@ -541,6 +550,9 @@ class Linear8(_Plugin):
 
     def __call__(self, q, scale, voxel_num, out_dtype=None, stream=None):
         """q float8_e4m3fn [max_voxels, in_channel], scale f32 [max_voxels, 1] -> [max_voxels, out_channel], FP16 unless said otherwise"""
+        if _another_stream(stream):
+            with _torch().cuda.stream(stream):
+                return self(q, scale, voxel_num, out_dtype)
         ins = (q, scale, voxel_num)
         _dense(*ins)
         out = q.new_empty((self.max_voxels, self.cout), dtype=out_dtype or _torch().float16)
@@ -579,6 +591,9 @@ class VoxelAttention(_Plugin):
         return obj
 
     def _enqueue_bound(self, bound, inputs, outputs, stream, workspace=None):
+        if workspace is None and self.ws is None and _another_stream(stream):
+            with _torch().cuda.stream(stream):
+                self._workspace(bound, inputs[0].device)
         self._list = super()._enqueue_bound(bound, inputs, outputs, stream, workspace)
         return self._list
 
@@ -598,6 +613,9 @@ class VoxelAttention(_Plugin):
     def __call__(self, qkv, coors, voxel_num, stream=None, windows_from=None):
         """qkv [max_voxels, (num_heads + 2 num_kv_heads) * head_dim] -> [max_voxels, num_heads * head_dim].  windows_from: a layer on
         the same coordinates and windows that has run on this stream."""
+        if _another_stream(stream):
+            with _torch().cuda.stream(stream):
+                return self(qkv, coors, voxel_num, windows_from=windows_from)
         ins = (qkv, coors, voxel_num)
         _dense(*ins)
         out = qkv.new_empty((self.max_voxels, self.cout))

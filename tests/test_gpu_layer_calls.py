@@ -147,3 +147,61 @@ def test_layers_read_back_from_their_bytes_are_called_as_the_first_ones():
     lin = api.Linear8(96, 40, rng.standard_normal((96, 40)).astype(np.float32), max_voxels=rows)
     lin.set_epilogue(None, rng.standard_normal(40).astype(np.float32), relu=True)
     assert torch.equal(api.Linear8.deserialize(lin.serialize())(*a, n), lin(*a, n))
+
+
+def test_a_call_on_another_stream_takes_no_memory_of_the_current_one():
+    """What was freed on the current stream may still be read there: outputs and workspaces of a call on another stream lie elsewhere."""
+    rng = np.random.default_rng(0)
+    rows = 5000
+    x, c, n = attention_inputs(rows)
+    q, s = linear_inputs(rows, 64)
+    norm = api.RmsNorm(96, rng.uniform(0.5, 1.5, 96).astype(np.float32), max_voxels=rows)
+    lin = api.Linear8(64, 160, rng.standard_normal((64, 160)).astype(np.float32), max_voxels=rows)
+    side = torch.cuda.Stream()
+    attn = attention(rows)
+    want = norm(x, n, x) + (lin(q, s, n), attn(x, c, n))
+    torch.cuda.synchronize()
+    fresh = [attention(rows) for _ in range(2)]
+    bytes_of = lambda t: t.untyped_storage().nbytes()  # noqa: E731
+    freed = set()
+    for t in [t for t in want + (attn.ws,) for _ in range(3)]:   # as large as what the calls below take
+        block = torch.empty(bytes_of(t), dtype=torch.uint8, device=DEV)
+        freed.add((block.data_ptr(), bytes_of(t)))
+        del block
+    side.wait_stream(torch.cuda.current_stream())
+    got = norm(x, n, x, stream=side) + (lin(q, s, n, stream=side), fresh[0](x, c, n, stream=side))
+    out = torch.empty_like(want[-1])
+    fresh[1].configure([x, c, n], [out])
+    fresh[1].enqueue([x, c, n], [out], side)
+    for t in got + tuple(f.ws for f in fresh):
+        a, b = t.data_ptr(), t.data_ptr() + bytes_of(t)
+        assert not any(a < p + size and p < b for p, size in freed)
+    assert torch.cuda.current_stream() != side
+    side.synchronize()
+    for a, b in zip(got + (out,), want + (want[-1],)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("rows", [1500, 6000])
+def test_shared_windows_in_one_graph(rows):
+    """A layer and a sharer of its windows, captured together and replayed on other frames."""
+    x, c, n = attention_inputs(rows)
+    first, second = attention(rows, slopes=[1.0, 2.0]), attention(rows, cap=20.0)
+    eager = attention(rows, slopes=[1.0, 2.0]), attention(rows, cap=20.0)
+    outs = [torch.empty((rows, 32), dtype=HALF, device=DEV) for _ in range(2)]
+    first(x, c, n)
+    second(x, c, n, windows_from=first)      # (workspace and descriptors are there)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        outs = first(x, c, n), second(x, c, n, windows_from=first)
+    for k, m in enumerate((rows, 7, 0, rows - 5)):
+        y, d, _ = attention_inputs(rows, seed=k)
+        x.copy_(y)
+        c.copy_(d)
+        n.fill_(m)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, op in zip(outs, eager):
+            assert torch.equal(got, op(x, c, n))
+        assert first.status() == second.status() == 0
